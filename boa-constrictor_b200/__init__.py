@@ -37,6 +37,7 @@ PROF_CLASSES = 12
 _u8p, _u32p, _u64p, _f32p = (C.POINTER(C.c_uint8), C.POINTER(C.c_uint32), C.POINTER(C.c_uint64),
                              C.POINTER(C.c_float))
 _i32p = C.POINTER(C.c_int32)
+_vp, _i64 = C.c_void_p, C.c_int64
 
 
 class BoaError(RuntimeError):
@@ -113,6 +114,19 @@ SIGNATURES = {
     "boa_pyrc_read": (C.c_int, [C.c_void_p, _u32p, _i32p, C.c_void_p]),
     "boa_pyrc_load": (C.c_int, [C.c_void_p, _u32p, _i32p, C.c_void_p]),
     "boa_pyrc_init_decoder": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "boa_embed": (C.c_int, [_vp, C.c_int, _i64, _vp, C.c_int, _i64, C.c_int, C.c_int, C.c_float, _vp, C.c_int, _i64,
+                            _vp]),
+    "boa_embed_backward_workspace": (C.c_size_t, [_i64, C.c_int, C.c_int]),
+    "boa_embed_backward": (C.c_int, [_vp, C.c_int, _i64, _vp, C.c_int, _i64, C.c_int, C.c_int, C.c_float, C.c_int,
+                                     _vp, C.c_int, _i64, _vp, C.c_size_t, _vp]),
+    "boa_mingru_states_floats": (C.c_uint64, [C.c_int, C.c_int, C.c_int]),
+    "boa_mingru_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "boa_mingru_scan": (C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _i64, _i64,
+                                  _vp, _vp, _vp, C.c_size_t, _vp]),
+    "boa_mingru_scan_backward": (C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _i64,
+                                           _i64, _vp, _vp, _i64, _i64, _vp, _vp, C.c_size_t, _vp]),
+    "boa_token_loss": (C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, _vp, C.c_int, C.c_float, _vp, C.c_float, _vp,
+                                 _vp, _i64, _vp]),
     "boa_pyrc_decode_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 

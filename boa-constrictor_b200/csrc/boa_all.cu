@@ -6,8 +6,12 @@
 #include "mlp.cu"
 #include "mamba.cu"
 #include "rnn.cu"
+#include "embed.cu"
+#include "recur.cu"
+#include "loss.cu"
 #include "runtime.cpp"
 #include "container.cpp"
 #include "noalloc.cu"
 #include "coder_api.cu"
 #include "pyrc.cu"
+#include "train_api.cu"

@@ -27,6 +27,10 @@ using bf16 = __nv_bfloat16;
 namespace {
 
 std::string g_load_error;  // boa_model_load failures (no handle yet)
+// Failures of the handle-free operators of train_api.cu, per thread: several
+// threads may make such calls at once.  Empty once a later handle-free call of
+// another kind fails in the thread, whose message then is the last one.
+thread_local char t_call_error[256] = "";
 
 // Makes `device` current for the scope of an API call and restores the
 // caller's current device afterwards: no entry point changes it.
@@ -198,7 +202,12 @@ boa_model::~boa_model() {
 namespace {
 
 int fail(boa_model* m, int code, const std::string& msg) {
-  if (m) m->err = msg; else g_load_error = msg;
+  if (m) {
+    m->err = msg;
+  } else {
+    g_load_error = msg;
+    t_call_error[0] = 0;
+  }
   return code;
 }
 int cuda_fail(boa_model* m, cudaError_t e, const char* where) {
@@ -542,7 +551,10 @@ uint32_t boa_stream_capacity_words(uint32_t chunk_len) {
   return (uint32_t)((bits + 31) / 32 + 8);
 }
 
-const char* boa_last_error(const boa_model* h) { return h ? h->err.c_str() : g_load_error.c_str(); }
+const char* boa_last_error(const boa_model* h) {
+  if (h) return h->err.c_str();
+  return t_call_error[0] ? t_call_error : g_load_error.c_str();
+}
 
 int boa_model_load(const char* path, int backbone, int d, int nl, int device, boa_model** out) {
   if (!out) return fail(nullptr, BOA_E_INVALID, "out is NULL");

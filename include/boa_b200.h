@@ -240,6 +240,89 @@ int boa_rc_decode_cdf_steps(void* d_states, const uint32_t* d_cdf, int n_streams
  * range_coder_kernels.cu:860-925 for testing.  Host buffers. */
 int boa_cdf_from_logits(boa_model* h, const float* logits, int rows, float inv_temperature, uint32_t* cdf);
 
+/* ---- operators for training and stepping a predictor ---------------------
+ * The parts of a byte predictor that are not plain matrix products, forward
+ * and backward, for callers that train the weights this library loads or that
+ * drive a predictor of their own next to the step-wise coder above.  No
+ * counterpart in the reference's C++ (its training is PyTorch).  They follow
+ * the step-wise coder: no handle, no allocation, every pointer a device
+ * pointer the caller owns (buffers of one call are on the current device),
+ * kernels only enqueued on `stream` (NULL = legacy default stream; a stream
+ * of another device is BOA_E_INVALID).  Every call can be captured into a
+ * CUDA graph.  Calls may run at once on several streams or threads as long as
+ * they share no output and no workspace.  A workspace is scratch of one call:
+ * its contents before and after mean nothing.  Buffers of a call do not
+ * overlap, except where in-place use is stated.  The message of a failed call
+ * is boa_last_error(NULL) in the calling thread.
+ *
+ * Element types (BOA_F32 ..) may differ where an argument names its own type;
+ * arithmetic is fp32 or wider and results are rounded once, to nearest.
+ * Buffers need the alignment of their element only; 16-byte aligned buffers
+ * and rows run fastest.  Results do not depend on timing: the same inputs on
+ * the same kind of GPU give the same bits. */
+#define BOA_F32 0
+#define BOA_F16 1
+#define BOA_BF16 2
+#define BOA_TOK_U8 0
+#define BOA_TOK_I32 1
+#define BOA_TOK_I64 2
+
+/* Embedding lookup: out[i][:] = scale * table[tokens[i]][:], i < n, rows of d
+ * elements ld_* elements apart; vocab <= 1024 rows (the largest alphabet of
+ * the coders).  A token outside [0, vocab) pads: its row is zeros. */
+int boa_embed(const void* d_tokens, int token_type, int64_t n, const void* d_table, int table_type, int64_t ld_table,
+              int vocab, int d, float scale, void* d_out, int out_type, int64_t ld_out, void* stream);
+/* Its gradient: dtable[v][:] = scale * sum of dout[i][:] over i with
+ * tokens[i] == v, plus the old dtable[v][:] when accumulate != 0.  Padding
+ * rows of dout are not read.  The rows are summed in token order (a stable
+ * sort), without atomics on the sums. */
+size_t boa_embed_backward_workspace(int64_t n, int vocab, int d);
+int boa_embed_backward(const void* d_tokens, int token_type, int64_t n, const void* d_dout, int dout_type,
+                       int64_t ld_dout, int vocab, int d, float scale, int accumulate, void* d_dtable,
+                       int dtable_type, int64_t ld_dtable, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* The minGRU recurrence (BOA_BACKBONE_MINGRU's cell) over T positions of
+ * n_chunks chunks.  Position t of chunk b is the row of 2d elements at
+ * zh + b * zh_chunk + t * zh_row: d gate logits zl, then d candidates hr.
+ *   z = sigmoid(zl); c = hr >= 0 ? hr + 1/2 : sigmoid(hr)
+ *   h[b][t] = (1 - z) h[b][t-1] + z c
+ * d_lengths (NULL = all T) gives each chunk's positions, clamped to 0 .. T:
+ * rows of zh at or past it are not read, and rows of h there are zeros.  d_h0
+ * [n_chunks][d] (NULL = zeros) is the state before position 0, d_h_last (may
+ * be NULL; may be d_h0) receives the state after the last position.  With
+ * T = 1 this is the decode step.  d_states, when not NULL, receives
+ * boa_mingru_states_floats floats that the backward call needs; their layout
+ * is the library's own.  T = 0 only moves the state. */
+uint64_t boa_mingru_states_floats(int n_chunks, int T, int d);
+size_t boa_mingru_workspace(int n_chunks, int T, int d);
+int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
+                    const int32_t* d_lengths, const float* d_h0, void* d_h, int64_t h_row, int64_t h_chunk,
+                    float* d_h_last, float* d_states, void* d_workspace, size_t workspace_bytes, void* stream);
+/* Its gradient, for the same zh, type, sizes and lengths and the d_states of
+ * the forward call: from dh [b][t] and d_dh_last (NULL = zeros) to dzh [b][t]
+ * (2d elements a row) and d_dh0 (may be NULL; may be d_dh_last).  Rows of dh
+ * at or past a chunk's length are not read, rows of dzh there are zeros. */
+int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
+                             const int32_t* d_lengths, const float* d_states, const void* d_dh, int64_t dh_row,
+                             int64_t dh_chunk, const float* d_dh_last, void* d_dzh, int64_t dzh_row,
+                             int64_t dzh_chunk, float* d_dh0, void* d_workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* Next-token cross entropy of n_rows rows of vocab <= 1024 logits, and its
+ * gradient, in one pass:
+ *   loss[i] = -ln p[target], p = softmax(inv_temperature * logits[i])
+ *   dlogits[i] = grad_scale * (d_dloss ? d_dloss[i] : 1) * inv_temperature
+ *                * (p - onehot(target))
+ * loss is in nats (times 1 / ln 2 = the bits the coder would spend, up to its
+ * quantiser).  d_loss or d_dlogits may be NULL, not both; d_dlogits has the
+ * logits' type and may be d_logits (same ld).  A target outside [0, vocab)
+ * pads: its logits are not read, loss and gradient are 0.  A masked logit
+ * (-inf or the type's lowest value) has p = 0; a row of -inf alone has loss
+ * +inf and gradient 0; NaN or +inf in a row makes that row's results NaN. */
+int boa_token_loss(const void* d_logits, int type, int64_t ld, int64_t n_rows, int vocab, const void* d_targets,
+                   int token_type, float inv_temperature, const float* d_dloss, float grad_scale, float* d_loss,
+                   void* d_dlogits, int64_t ld_dlogits, void* stream);
+
 /* ---- BOA2 container (boa.cpp:85-107, :158-277, :538-581) ----------------
  * Serialises a container into buf (cap bytes); *len_out = bytes needed (call
  * with buf = NULL to size).  flags bit0 = warm start; interleave_batch is
