@@ -120,11 +120,10 @@ SIGNATURES = {
     "boa_embed_backward": (C.c_int, [_vp, C.c_int, _i64, _vp, C.c_int, _i64, C.c_int, C.c_int, C.c_float, C.c_int,
                                      _vp, C.c_int, _i64, _vp, C.c_size_t, _vp]),
     "boa_mingru_states_floats": (C.c_uint64, [C.c_int, C.c_int, C.c_int]),
-    "boa_mingru_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "boa_mingru_scan": (C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _i64, _i64,
-                                  _vp, _vp, _vp, C.c_size_t, _vp]),
+                                  _vp, _vp, _vp]),
     "boa_mingru_scan_backward": (C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _i64,
-                                           _i64, _vp, _vp, _i64, _i64, _vp, _vp, C.c_size_t, _vp]),
+                                           _i64, _vp, _vp, _i64, _i64, _vp, _vp]),
     "boa_token_loss": (C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, _vp, C.c_int, C.c_float, _vp, C.c_float, _vp,
                                  _vp, _i64, _vp]),
     "boa_pyrc_decode_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),

@@ -99,14 +99,9 @@ uint64_t boa_mingru_states_floats(int n_chunks, int T, int d) {
   if (n_chunks < 0 || T < 0 || d < 1 || d > boa::kMaxWidth) return 0;
   return boa::mingru_states_floats(n_chunks, T, d);
 }
-size_t boa_mingru_workspace(int n_chunks, int T, int d) {
-  if (n_chunks < 0 || T < 0 || d < 1 || d > boa::kMaxWidth) return 0;
-  return boa::mingru_workspace(n_chunks, T, d);
-}
-
 int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
                     const int32_t* d_lengths, const float* d_h0, void* d_h, int64_t h_row, int64_t h_chunk,
-                    float* d_h_last, float* d_states, void* d_workspace, size_t workspace_bytes, void* stream) {
+                    float* d_h_last, float* d_states, void* stream) {
   BOA_REQUIRE(type_ok(type), "unknown element type");
   BOA_REQUIRE(n_chunks >= 0 && T >= 0, "negative size");
   BOA_REQUIRE(d >= 1 && d <= boa::kMaxWidth, "d must be 1 .. 65536");
@@ -118,19 +113,15 @@ int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk
   BOA_REQUIRE(elem_aligned(d_zh, type) && elem_aligned(d_h, type) && boa::aligned_to(d_lengths, 4) &&
                   boa::aligned_to(d_h0, 4) && boa::aligned_to(d_h_last, 4) && boa::aligned_to(d_states, 4),
               "a buffer is not aligned to its element");
-  const size_t need = boa::mingru_workspace(n_chunks, T, d);
-  BOA_REQUIRE(need == 0 || (d_workspace && boa::aligned_to(d_workspace, 16) && workspace_bytes >= need),
-              "the workspace is null, not aligned to 16 bytes or below boa_mingru_workspace");
   return train_launch(__func__, boa::launch_mingru_scan(d_zh, type, {zh_row, zh_chunk}, n_chunks, T, d, d_lengths,
-                                                        d_h0, d_h, {h_row, h_chunk}, d_h_last, d_states, d_workspace,
+                                                        d_h0, d_h, {h_row, h_chunk}, d_h_last, d_states,
                                                         (cudaStream_t)stream));
 }
 
 int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
                              const int32_t* d_lengths, const float* d_states, const void* d_dh, int64_t dh_row,
                              int64_t dh_chunk, const float* d_dh_last, void* d_dzh, int64_t dzh_row,
-                             int64_t dzh_chunk, float* d_dh0, void* d_workspace, size_t workspace_bytes,
-                             void* stream) {
+                             int64_t dzh_chunk, float* d_dh0, void* stream) {
   BOA_REQUIRE(type_ok(type), "unknown element type");
   BOA_REQUIRE(n_chunks >= 0 && T >= 0, "negative size");
   BOA_REQUIRE(d >= 1 && d <= boa::kMaxWidth, "d must be 1 .. 65536");
@@ -144,13 +135,9 @@ int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t
                   boa::aligned_to(d_lengths, 4) && boa::aligned_to(d_states, 4) && boa::aligned_to(d_dh_last, 4) &&
                   boa::aligned_to(d_dh0, 4),
               "a buffer is not aligned to its element");
-  const size_t need = boa::mingru_workspace(n_chunks, T, d);
-  BOA_REQUIRE(need == 0 || (d_workspace && boa::aligned_to(d_workspace, 16) && workspace_bytes >= need),
-              "the workspace is null, not aligned to 16 bytes or below boa_mingru_workspace");
   return train_launch(__func__, boa::launch_mingru_scan_grad(d_zh, type, {zh_row, zh_chunk}, n_chunks, T, d,
                                                              d_lengths, d_states, d_dh, {dh_row, dh_chunk}, d_dh_last,
-                                                             d_dzh, {dzh_row, dzh_chunk}, d_dh0, d_workspace,
-                                                             (cudaStream_t)stream));
+                                                             d_dzh, {dzh_row, dzh_chunk}, d_dh0, (cudaStream_t)stream));
 }
 
 int boa_token_loss(const void* d_logits, int type, int64_t ld, int64_t n_rows, int vocab, const void* d_targets,

@@ -5,6 +5,9 @@
 // once, to nearest, when it is stored.
 #pragma once
 #include <cstdint>
+#include <initializer_list>
+#include <type_traits>
+#include <utility>
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -85,13 +88,12 @@ struct RowStrides {
 
 // minGRU over T positions per chunk; see recur.cu
 size_t mingru_states_floats(int B, int T, int d);
-size_t mingru_workspace(int B, int T, int d);
 cudaError_t launch_mingru_scan(const void* zh, int type, RowStrides zs, int B, int T, int d, const int* lengths,
-                               const float* h0, void* h, RowStrides hs, float* h_last, float* states, void* ws,
+                               const float* h0, void* h, RowStrides hs, float* h_last, float* states,
                                cudaStream_t st);
 cudaError_t launch_mingru_scan_grad(const void* zh, int type, RowStrides zs, int B, int T, int d, const int* lengths,
                                     const float* states, const void* dh, RowStrides dhs, const float* dh_last,
-                                    void* dzh, RowStrides dzs, float* dh0, void* ws, cudaStream_t st);
+                                    void* dzh, RowStrides dzs, float* dh0, cudaStream_t st);
 
 // Next-token cross entropy per row and its gradient; see loss.cu
 cudaError_t launch_token_loss(const void* logits, int type, long long ld, long long rows, int vocab,

@@ -193,11 +193,8 @@ def mingru_scan(zh, h0=None, lengths=None, out=None, h_last=None, save_states: b
     states = None
     if save_states:
         states = torch.empty(L.boa_mingru_states_floats(B, T, d), dtype=torch.float32, device=device)
-    need = L.boa_mingru_workspace(B, T, d)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call(L.boa_mingru_scan, device, zh.data_ptr(), _type(zh, "zh"), zh.stride(1), zh.stride(0), B, T, d,
-          _ptr(lengths), _ptr(h0), out.data_ptr(), out.stride(1), out.stride(0), h_last.data_ptr(), _ptr(states),
-          _ptr(ws), need)
+          _ptr(lengths), _ptr(h0), out.data_ptr(), out.stride(1), out.stride(0), h_last.data_ptr(), _ptr(states))
     return (out, h_last, states) if save_states else (out, h_last)
 
 
@@ -223,11 +220,9 @@ def mingru_scan_backward(zh, states, dh, dh_last=None, lengths=None, out=None):
     dh_last = _state(dh_last, B, d, device, "dh_last")
     dh0 = torch.empty((B, d), dtype=torch.float32, device=device)
     lengths = _lengths(lengths, B, device)
-    need = L.boa_mingru_workspace(B, T, d)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     _call(L.boa_mingru_scan_backward, device, zh.data_ptr(), _type(zh, "zh"), zh.stride(1), zh.stride(0), B, T, d,
           _ptr(lengths), states.data_ptr(), dh.data_ptr(), dh.stride(1), dh.stride(0), _ptr(dh_last),
-          out.data_ptr(), out.stride(1), out.stride(0), dh0.data_ptr(), _ptr(ws), need)
+          out.data_ptr(), out.stride(1), out.stride(0), dh0.data_ptr())
     return out, dh0
 
 

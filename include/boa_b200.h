@@ -294,10 +294,9 @@ int boa_embed_backward(const void* d_tokens, int token_type, int64_t n, const vo
  * boa_mingru_states_floats floats that the backward call needs; their layout
  * is the library's own.  T = 0 only moves the state. */
 uint64_t boa_mingru_states_floats(int n_chunks, int T, int d);
-size_t boa_mingru_workspace(int n_chunks, int T, int d);
 int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
                     const int32_t* d_lengths, const float* d_h0, void* d_h, int64_t h_row, int64_t h_chunk,
-                    float* d_h_last, float* d_states, void* d_workspace, size_t workspace_bytes, void* stream);
+                    float* d_h_last, float* d_states, void* stream);
 /* Its gradient, for the same zh, type, sizes and lengths and the d_states of
  * the forward call: from dh [b][t] and d_dh_last (NULL = zeros) to dzh [b][t]
  * (2d elements a row) and d_dh0 (may be NULL; may be d_dh_last).  Rows of dh
@@ -305,8 +304,7 @@ int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk
 int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
                              const int32_t* d_lengths, const float* d_states, const void* d_dh, int64_t dh_row,
                              int64_t dh_chunk, const float* d_dh_last, void* d_dzh, int64_t dzh_row,
-                             int64_t dzh_chunk, float* d_dh0, void* d_workspace, size_t workspace_bytes,
-                             void* stream);
+                             int64_t dzh_chunk, float* d_dh0, void* stream);
 
 /* Next-token cross entropy of n_rows rows of vocab <= 1024 logits, and its
  * gradient, in one pass:

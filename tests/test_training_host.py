@@ -19,15 +19,13 @@ def _embed_bwd(L, tok_t=0, n=8, g_t=0, ld_g=16, vocab=256, d=16, t_t=0, ld_t=16,
     return L.boa_embed_backward(p[0], tok_t, n, p[1], g_t, ld_g, vocab, d, 1.0, 0, p[2], t_t, ld_t, p[3], ws, None)
 
 
-def _scan(L, t=0, zr=32, zc=320, B=4, T=10, d=16, hr=16, hc=160, zh=A, h=A, h0=None, ws=None):
-    ws = L.boa_mingru_workspace(B, T, d) if ws is None else ws
-    return L.boa_mingru_scan(zh, t, zr, zc, B, T, d, None, h0, h, hr, hc, None, None, A, ws, None)
+def _scan(L, t=0, zr=32, zc=320, B=4, T=10, d=16, hr=16, hc=160, zh=A, h=A, h0=None):
+    return L.boa_mingru_scan(zh, t, zr, zc, B, T, d, None, h0, h, hr, hc, None, None, None)
 
 
-def _scan_bwd(L, t=0, zr=32, zc=320, B=4, T=10, d=16, gr=16, gc=160, dr=32, dc=320, p=(A, A, A, A), ws=None):
-    ws = L.boa_mingru_workspace(B, T, d) if ws is None else ws
+def _scan_bwd(L, t=0, zr=32, zc=320, B=4, T=10, d=16, gr=16, gc=160, dr=32, dc=320, p=(A, A, A, A)):
     return L.boa_mingru_scan_backward(p[0], t, zr, zc, B, T, d, None, p[1], p[2], gr, gc, None, p[3], dr, dc, None,
-                                      A, ws, None)
+                                      None)
 
 
 def _loss(L, t=0, ld=256, rows=8, vocab=256, tok_t=0, inv=1.0, ld_g=256, p=(A, A, A, C.c_void_p(512))):
