@@ -33,10 +33,20 @@
 namespace boa {
 
 constexpr int kSpan = 32;         // positions between two saved states
-constexpr int kMaxWarps = 16;     // warps of a block
+constexpr int kMaxWarps = 16;    // warps of a block
 constexpr int kMaxCluster = 8;    // blocks of a cluster (the portable limit)
-constexpr int kScanSteps = 8;     // positions a warp holds, forward
-constexpr int kGradSteps = 4;     // and backward, which holds twice the values
+constexpr int kFew = 8;           // up to here, one thread takes a chain through all positions
+// Positions that a warp holds, and registers a thread, for V chains a lane.
+// Longer runs spread the exchange over more positions; fewer registers let
+// more warps hide each other's latencies.  Four-byte pairs have the bytes to
+// wait for, so there the warps win (256 x 1024 x 256 forward: 4 positions at 56
+// registers 143 us, 8 at 80 169 us); two-byte pairs are paced by instructions
+// (64 x 4096 x 256 forward: 165 us and 129 us).
+template <typename T_, int V>
+constexpr int scan_steps() { return V == 2 && sizeof(T_) == 4 ? 4 : 8; }
+template <typename T_, int V>
+constexpr int scan_regs() { return V == 2 && sizeof(T_) == 4 ? 56 : 80; }
+constexpr int kGradSteps = 8, kGradRegs = 112;
 
 // n / d for n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and
 // mul = floor(2^(31+s) / d) + 1, mul d exceeds 2^(31+s) by at most d, and
@@ -64,25 +74,74 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return y;
 }
 
-// The cell's gates.  Both sigmoids are taken of -|x|, so the exponentials are
-// at most 1, the smaller of z and 1 - z comes without a cancellation, and one
-// reciprocal of the two denominators' product (1 .. 4) serves both: three
-// special-function operations instead of four, which would run out before HBM
-// does with 16-bit gates.  The larger of z and 1 - z is 1 minus the smaller,
-// so a closed gate keeps the state exactly, however many positions long.
-struct Cell {
-  float a, z, c;
+// V chains of a lane.  (Packed pairs, f32x2, were measured slower: they run on
+// one of the two FMA pipes only, and most of the arithmetic here is FMA work.)
+template <int V>
+struct Vec {
+  float v[V];
 };
-__device__ __forceinline__ Cell mingru_cell(float zl, float hr) {
+template <int V>
+__device__ __forceinline__ Vec<V> all_of(float x) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = x;
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> vfma(const Vec<V>& a, const Vec<V>& b, const Vec<V>& c) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = __fmaf_rn(a.v[i], b.v[i], c.v[i]);
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vec<V> vmul(const Vec<V>& a, const Vec<V>& b) {
+  Vec<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = __fmul_rn(a.v[i], b.v[i]);
+  return r;
+}
+
+__device__ __forceinline__ float max_or_nan(float x, float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
+// The cell's gates for V chains.  One reciprocal of both denominators'
+// product serves both sigmoids: three special-function operations an element
+// instead of four.  With e = exp(-zl), f = exp(-|hr|), p = 1 + e, q = 1 + f and
+// r = 1 / (p q):
+//
+//   z = q r = f r + r     sigmoid(-|hr|) = f (p r)     a = 1 - z
+//
+// zl is cut off at -88, where p q stays below 2^128 and its reciprocal is
+// below 2^-126, which the instruction flushes: from there down z is 0 and
+// a is 1, exactly (the candidate then has no weight).  A closed gate so keeps
+// the state however many positions long.
+template <int V>
+struct Cell {
+  Vec<V> a, b;  // 1 - z, z c
+  Vec<V> z, w;  // z, z c'(hr): for the gradient
+};
+template <int V, bool GRAD>
+__device__ __forceinline__ Cell<V> mingru_cell(const Vec<V>& zl, const Vec<V>& hr) {
   constexpr float kLog2e = 1.44269504f;
-  const float e = ex2_fast(-fabsf(zl) * kLog2e), f = ex2_fast(-fabsf(hr) * kLog2e);
-  const float p = 1.f + e, q = 1.f + f;
-  const float r = rcp_fast(p * q);
-  const float small = e * (q * r), big = 1.f - small;  // e / p and 1 / p
-  Cell k;
-  k.z = zl >= 0.f ? big : small;
-  k.a = zl >= 0.f ? small : big;
-  k.c = hr >= 0.f ? hr + 0.5f : f * (p * r);
+  Cell<V> k;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float e = ex2_fast(max_or_nan(zl.v[v], -88.f) * -kLog2e), f = ex2_fast(fabsf(hr.v[v]) * -kLog2e);
+    const float p = 1.f + e;
+    const float r = rcp_fast(__fmaf_rn(p, f, p));
+    const float z = __fmaf_rn(f, r, r), low = f * (p * r);
+    // hr + 1/2 lies below sigmoid(hr) for hr < 0 (slopes 1 and at most 1/4
+    // from the same value at 0), and above sigmoid(-hr) <= 1/2 otherwise
+    const float c = fmaxf(hr.v[v] + 0.5f, low);
+    k.a.v[v] = 1.f - z;
+    k.b.v[v] = z * c;
+    k.z.v[v] = z;
+    if (GRAD) k.w.v[v] = z * (hr.v[v] >= 0.f ? 1.f : __fmaf_rn(-low, low, low));
+  }
   return k;
 }
 
@@ -92,38 +151,54 @@ size_t mingru_states_floats(int B, int T, int d) { return (size_t)spans_of(T) * 
 // The map of a run of positions for V chains: x -> A x + B.
 template <int V>
 struct alignas(8 * V) Map {
-  float A[V], B[V];
+  Vec<V> A, B;
 };
 template <int V>
-__device__ __forceinline__ Map<V> identity_map() {
-  Map<V> m;
-#pragma unroll
-  for (int v = 0; v < V; ++v) { m.A[v] = 1.f; m.B[v] = 0.f; }
-  return m;
-}
-template <int V>
-__device__ __forceinline__ void apply(const Map<V>& m, float (&x)[V]) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) x[v] = __fmaf_rn(m.A[v], x[v], m.B[v]);
-}
+__device__ __forceinline__ Vec<V> apply(const Map<V>& m, const Vec<V>& x) { return vfma(m.A, x, m.B); }
 // m, then n
 template <int V>
-__device__ __forceinline__ void then(Map<V>& m, const Map<V>& n) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    m.B[v] = __fmaf_rn(n.A[v], m.B[v], n.B[v]);
-    m.A[v] *= n.A[v];
-  }
+__device__ __forceinline__ Map<V> then(const Map<V>& m, const Map<V>& n) {
+  return {vmul(m.A, n.A), vfma(n.A, m.B, n.B)};
 }
 
-// Shared memory of a walk.  Everything is double-buffered by the step's
-// parity: what a step writes was last read two steps ago, and every warp
-// passes one barrier in between.
+// Shared memory of a walk, for a block of `warps` warps.  Everything is
+// double-buffered by the step's parity: what a step writes was last read two
+// steps ago, and every warp passes one barrier in between.
 template <int V>
 struct Walk {
-  Map<V> warp[2][kMaxWarps][32];      // the warps' maps
-  Map<V> block[2][kMaxCluster][32];   // the cluster's blocks' maps (pushed by their owners)
-  float state[2][kMaxWarps][32][V];   // the walk's state, left by the group's last warp (no cluster)
+  Map<V>* maps;     // [2][warps][32]: the warps' maps
+  Map<V>* forward;  // [2][warps][32]: backward, their maps of the state
+  Map<V>* block;    // [2][ranks][32]: the cluster's blocks' maps, pushed by their owners (ranks > 1)
+  Vec<V>* state;    // [2][32]: the walk's state, left by the last warp (ranks = 1)
+  uint64_t* full;   // [2]: barriers that count the bytes pushed into `block` (ranks > 1)
+  uint8_t* stages;
+  int warps, ranks;
+  __device__ __forceinline__ Walk(uint8_t* at, int ranks_, bool both) : warps(blockDim.x >> 5), ranks(ranks_) {
+    maps = reinterpret_cast<Map<V>*>(at);
+    forward = maps + 64 * warps;
+    block = forward + (both ? 64 * warps : 0);
+    state = reinterpret_cast<Vec<V>*>(block + (ranks > 1 ? 64 * ranks : 0));
+    full = reinterpret_cast<uint64_t*>(state + 64);
+    stages = reinterpret_cast<uint8_t*>(full + 2);
+  }
+  static size_t bytes(int warps, int ranks, bool both) {
+    return sizeof(Map<V>) * 64 * ((both ? 2 : 1) * warps + (ranks > 1 ? ranks : 0)) + sizeof(Vec<V>) * 64 + 16;
+  }
+  // Called by all threads before anything else; afterwards the cluster's
+  // blocks have started and their barriers are ready.
+  __device__ __forceinline__ void start() const {
+    if (ranks == 1) return;
+    if (threadIdx.x == 0) {
+      mbar_init(full, 1);
+      mbar_init(full + 1, 1);
+      fence_mbar_init();
+    }
+    cluster_sync_all();
+  }
+  // No block leaves before the others' last pushes have gone out.
+  __device__ __forceinline__ void finish() const {
+    if (ranks > 1) cluster_sync_all();
+  }
 };
 
 // Where a warp works.  A block's warps form groups of `warps` (a power of
@@ -153,256 +228,425 @@ __device__ __forceinline__ Place place_of(int warps, int ranks, long long chains
   return p;
 }
 
+// Writes a map into another block's shared memory; its bytes are counted on
+// that block's barrier.  The barrier, and not a release by this block, says
+// that the map is there: a release would also wait for the block's stores to
+// HBM, a full memory latency in every step.
 template <int V>
-__device__ __forceinline__ void store_map_cluster(uint32_t addr, const Map<V>& m) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr + 4 * v), "f"(m.A[v]) : "memory");
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr + 4 * (V + v)), "f"(m.B[v]) : "memory");
+__device__ __forceinline__ void push_map(uint32_t addr, const Map<V>& m, uint32_t bar) {
+  if constexpr (V == 1)
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(addr),
+                 "f"(m.A.v[0]), "f"(m.B.v[0]), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::
+                     "r"(addr), "f"(m.A.v[0]), "f"(m.A.v[V - 1]), "f"(m.B.v[0]), "f"(m.B.v[V - 1]), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// false when the wait ran out: the walk's state is then NaN, and the walk goes
+// on without waiting again (a handle-free call has no error word to set)
+__device__ __forceinline__ bool await_maps(uint32_t bar, uint32_t parity) {
+  bool there = try_wait_cluster(bar, parity);
+  if (!there) {
+    const uint64_t t0 = global_ns();
+    while (!(there = try_wait_cluster(bar, parity)) && global_ns() - t0 <= kWaitLimitNs) {}
   }
+  __syncwarp();  // lanes may leave the loop apart
+  return there;
 }
 
 // One step's exchange.  `mine`: the map of this warp's positions, `x`: the
-// walk's state before the step; afterwards `s` is the state before this warp's
-// positions, and (in a cluster) `x` the state after the step.  REVERSE runs
-// from the last warp and block to the first.  Without a cluster the caller
-// hands the state on through leave().
+// walk's state before the step.  Returns the state before this warp's
+// positions; in a cluster x becomes the state after the step.  REVERSE runs
+// from the last warp and block to the first.  Without a cluster the state
+// after the step is handed on through leave().
+//
+// In a cluster, a slot of `block` is written again two steps on.  Its writer
+// has then seen this block's map of the step between, which goes out after
+// the barrier below, that is after all warps here have read the slot.
 template <int V, bool REVERSE>
-__device__ __forceinline__ void exchange(Walk<V>& K, const Place& p, int parity, const Map<V>& mine, float (&x)[V],
-                                         float (&s)[V], bool first_step) {
+__device__ __forceinline__ Vec<V> exchange(const Walk<V>& K, const Place& p, int step, const Map<V>& mine, Vec<V>& x,
+                                           bool& waiting) {
+  const int parity = step & 1;
   const int order = REVERSE ? p.warps - 1 - p.warp : p.warp;  // place of this warp along the walk
-  Map<V>(*maps)[32] = K.warp[parity] + p.first;
-  maps[order][p.lane] = mine;
+  Map<V>* maps = K.maps + (parity * K.warps + p.first) * 32 + p.lane;
+  maps[order * 32] = mine;
   __syncthreads();
+  Vec<V> s;
   if (p.ranks == 1) {
-    if (!first_step)
-#pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = K.state[parity][p.first][p.lane][v];
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = x[v];
+    s = step == 0 ? x : K.state[parity * 32 + p.lane];
   } else {
+    const uint32_t bar = smem_u32(K.full + parity);
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(K.full + parity, (uint32_t)(p.ranks * 32 * sizeof(Map<V>)));
     const int turn = REVERSE ? p.ranks - 1 - p.rank : p.rank;
     if (p.warp < p.ranks) {  // warp r takes the block's map to block r
-      Map<V> all = maps[0][p.lane];
-      for (int w = 1; w < p.warps; ++w) then<V>(all, maps[w][p.lane]);
-      store_map_cluster<V>(cluster_addr(&K.block[parity][turn][p.lane], (uint32_t)p.warp), all);
+      Map<V> all = maps[0];
+      for (int w = 1; w < p.warps; ++w) all = then<V>(all, maps[w * 32]);
+      push_map<V>(cluster_addr(K.block + (parity * p.ranks + turn) * 32 + p.lane, (uint32_t)p.warp), all,
+                  cluster_addr(K.full + parity, (uint32_t)p.warp));
     }
-    cluster_sync_all();
+    if (waiting && !await_maps(bar, (uint32_t)(step >> 1) & 1u)) {
+      waiting = false;
+      x = all_of<V>(__int_as_float(0x7fffffff));
+    }
     for (int r = 0; r < p.ranks; ++r) {
-      if (r == turn)
-#pragma unroll
-        for (int v = 0; v < V; ++v) s[v] = x[v];
-      apply<V>(K.block[parity][r][p.lane], x);
+      if (r == turn) s = x;
+      x = apply<V>(K.block[(parity * p.ranks + r) * 32 + p.lane], x);
     }
   }
-  for (int w = 0; w < order; ++w) apply<V>(maps[w][p.lane], s);
+#pragma unroll 4
+  for (int w = 0; w < order; ++w) s = apply<V>(maps[w * 32], s);
+  return s;
 }
 // The state after the step, for the next one (no cluster): the group's last
 // warp along the walk has it.
 template <int V, bool REVERSE>
-__device__ __forceinline__ void leave(Walk<V>& K, const Place& p, int parity, const float (&s)[V]) {
-  if (p.ranks == 1 && (REVERSE ? p.warp == 0 : p.warp == p.warps - 1))
-#pragma unroll
-    for (int v = 0; v < V; ++v) K.state[parity ^ 1][p.first][p.lane][v] = s[v];
+__device__ __forceinline__ void leave(const Walk<V>& K, const Place& p, int parity, const Vec<V>& s) {
+  if (p.ranks == 1 && (REVERSE ? p.warp == 0 : p.warp == p.warps - 1)) K.state[(parity ^ 1) * 32 + p.lane] = s;
 }
 
-// P rows of V elements from `x`, the first `live` of them; the others as `fill`
-template <int P, typename T_, int V>
-__device__ __forceinline__ void load_rows(Pack<T_, V> (&to)[P], const T_* x, long long row, int live, float fill) {
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    if (p < live) {
-      to[p] = *reinterpret_cast<const Pack<T_, V>*>(x + p * row);
+// Rows on their way from HBM: every lane copies the packs that it will use
+// itself into its own places of shared memory, so only its own copies need to
+// be waited for.  A pack of 2 bytes (odd widths) is too small for an
+// asynchronous copy and is moved by a load and a store.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+  if constexpr (BYTES >= 4) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+  } else {
+    const unsigned short x = __ldg(static_cast<const unsigned short*>(from));
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(x) : "memory");
+  }
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Packs as fp32 and back.  Pairs of 16 bits are taken as the 32-bit word that
+// they are: taken as two halves they cost twice the instructions.
+template <typename T_, int V>
+__device__ __forceinline__ Vec<V> widen(const Pack<T_, V>& p) {
+  Vec<V> r;
+  if constexpr (V == 2 && sizeof(T_) == 2) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&p);
+    if constexpr (std::is_same<T_, __nv_bfloat16>::value) {
+      r.v[0] = __uint_as_float(w << 16);
+      r.v[1] = __uint_as_float(w & 0xffff0000u);
     } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) to[p].v[v] = from_f32<T_>(fill);
+      __half2 h;
+      *reinterpret_cast<uint32_t*>(&h) = w;
+      const float2 f = __half22float2(h);
+      r.v[0] = f.x;
+      r.v[1] = f.y;
     }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) r.v[v] = to_f32(p.v[v]);
+  }
+  return r;
+}
+// a row that is not there as `fill`
+template <typename T_, int V>
+__device__ __forceinline__ Vec<V> widen(const Pack<T_, V>& p, bool there, float fill) {
+  Vec<V> r = widen(p);
+#pragma unroll
+  for (int v = 0; v < V; ++v) r.v[v] = there ? r.v[v] : fill;
+  return r;
+}
+template <typename T_, int V>
+__device__ __forceinline__ void store_rounded(T_* to, const Vec<V>& x) {
+  if constexpr (V == 2 && sizeof(T_) == 2) {
+    uint32_t w;
+    if constexpr (std::is_same<T_, __nv_bfloat16>::value) {
+      const __nv_bfloat162 r = __floats2bfloat162_rn(x.v[0], x.v[1]);
+      w = *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+      const __half2 r = __floats2half2_rn(x.v[0], x.v[1]);
+      w = *reinterpret_cast<const uint32_t*>(&r);
+    }
+    *reinterpret_cast<uint32_t*>(to) = w;
+  } else {
+    Pack<T_, V> p;
+#pragma unroll
+    for (int v = 0; v < V; ++v) p.v[v] = from_f32<T_>(x.v[v]);
+    *reinterpret_cast<Pack<T_, V>*>(to) = p;
   }
 }
 
-// Positions that are not a chunk's get a gate logit of -inf: a = 1 and z = 0
-// exactly, which leaves the state alone.
+// A lane's packs of a stage: [stream][P][32] of its warp, so that the offsets
+// of the rows are constants.
+template <typename T_, int V, int P, int STREAMS>
+__device__ __forceinline__ Pack<T_, V>* warp_stages(uint8_t* stages, int S) {
+  return reinterpret_cast<Pack<T_, V>*>(stages) + (threadIdx.x >> 5) * (S * STREAMS * P * 32) + (threadIdx.x & 31);
+}
+// row p after `x`, `row` bytes each: one multiply-add of 32 bits to 64
+template <typename P_>
+__device__ __forceinline__ P_* row_at(P_* x, uint32_t row, int p) {
+  using B_ = typename std::conditional<std::is_const<P_>::value, const char, char>::type;
+  return reinterpret_cast<P_*>(reinterpret_cast<B_*>(x) + (unsigned long long)row * (uint32_t)p);
+}
+template <int P, typename T_, int V>
+__device__ __forceinline__ void copy_rows(Pack<T_, V>* to, const T_* x, uint32_t row, int live, bool whole) {
+  const uint32_t at = smem_u32(to);
+  if (whole) {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      copy_async<sizeof(T_) * V>(at + p * 32 * (int)sizeof(Pack<T_, V>), row_at(x, row, p));
+  } else {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (p < live) copy_async<sizeof(T_) * V>(at + p * 32 * (int)sizeof(Pack<T_, V>), row_at(x, row, p));
+  }
+}
+// rows of [from, from + P) before `end`
+template <int P>
+__device__ __forceinline__ int rows_left(int from, int end) { return max(min(P, end - from), 0); }
+
+constexpr int kStages = 2;  // the step in use, and the next one on its way
+
+// Positions that are not a chunk's get a gate logit of -inf: a = 1 and b = 0
+// exactly, which leaves the state alone.  (p r = 0 there, and so is f (p r).)
+// A warp whose rows are all there (`whole`, the same for its lanes) takes a
+// form without those tests.
 // ------------------------------------------------------------------ forward
 template <typename T_, int V>
-__global__ void __launch_bounds__(kMaxWarps * 32, V == 1 ? 2 : 1)
-mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains, int warps,
-                   int ranks, const int* __restrict__ lengths, const float* h0, T_* __restrict__ h, RowStrides hs,
-                   float* h_last, float* __restrict__ states) {
-  constexpr int P = kScanSteps;
-  __shared__ Walk<V> K;
-  if (ranks > 1) cluster_sync_all();  // the others' shared memory is there from here on
+__global__ void __maxnreg__((scan_regs<T_, V>()))
+mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains,
+                   const int* __restrict__ lengths, const float* h0, T_* __restrict__ h, RowStrides hs,
+                   float* h_last, float* __restrict__ states, int warps, int ranks) {
+  constexpr int P = scan_steps<T_, V>(), S = kStages, STAGE = 2 * P * 32;
+  extern __shared__ __align__(16) uint8_t walk_smem[];
+  const Walk<V> K(walk_smem, ranks, false);
+  K.start();
   const Place at = place_of<V>(warps, ranks, chains, d, by_d);
   int len = at.in ? T : 0;
   if (at.in && lengths) len = min(max(lengths[at.b], 0), T);
+  const int end = at.in ? T : 0;
+  const int all_len = __reduce_min_sync(~0u, len);  // positions that all of the warp's chains have
   const int step = ranks * warps * P;  // positions of a step of the walk
-  long long t = (long long)(at.rank * warps + at.warp) * P;
+  int t = (at.rank * warps + at.warp) * P;
   const T_* x = zh + at.b * zs.chunk + t * zs.row + at.c;
   T_* o = h + at.b * hs.chunk + t * hs.row + at.c;
-  Pack<T_, V> zl[P], hr[P];
-  auto count = [&](int end, long long from) { return (int)max(min((long long)P, end - from), 0ll); };
-  int live = count(len, t);
-  load_rows(zl, x, zs.row, live, -INFINITY);
-  load_rows(hr, x + d, zs.row, live, 0.f);
-  float s[V], walk[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) walk[v] = at.in && h0 ? h0[at.chain + v] : 0.f;
+  Pack<T_, V>* const stages = warp_stages<T_, V, P, 2>(K.stages, S);
+  const long long x_step = step * zs.row, o_step = step * hs.row;
+  const uint32_t x_row = (uint32_t)(zs.row * sizeof(T_)), o_row = (uint32_t)(hs.row * sizeof(T_));
   const int steps = (T + step - 1) / step;
-  for (int i = 0; i < steps; ++i) {
-    float ga[P][V], gb[P][V];
-    Map<V> m = identity_map<V>();
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const Cell k = mingru_cell(to_f32(zl[p].v[v]), to_f32(hr[p].v[v]));
-        ga[p][v] = k.a;
-        gb[p][v] = k.z * k.c;
-        m.B[v] = __fmaf_rn(k.a, m.B[v], gb[p][v]);
-        m.A[v] *= k.a;
-      }
-    const int rows = at.in ? count(T, t) : 0, was = live;
-    if (i + 1 < steps) {
-      x += step * zs.row;
-      live = count(len, t + step);
-      load_rows(zl, x, zs.row, live, -INFINITY);
-      load_rows(hr, x + d, zs.row, live, 0.f);
+  int t_next = t, put = 0, got = 0;  // the next step to fetch, its stage, and the stage in use
+  auto fetch = [&](bool more) {
+    if (more) {
+      const int live = rows_left<P>(t_next, len);
+      const bool whole = t_next + P <= all_len;
+      copy_rows<P>(stages + put * STAGE, x, x_row, live, whole);
+      copy_rows<P>(stages + put * STAGE + P * 32, x + d, x_row, live, whole);
+      x += x_step;
+      t_next += step;
+      put = put + 1 == S ? 0 : put + 1;
     }
-    exchange<V, false>(K, at, i & 1, m, walk, s, i == 0);
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch(i < steps);
+  Vec<V> walk = all_of<V>(0.f), s = walk;
+  bool waiting = true;
+  if (at.in && h0)
+#pragma unroll
+    for (int v = 0; v < V; ++v) walk.v[v] = h0[at.chain + v];
+  for (int i = 0; i < steps; ++i) {
+    copies_wait<S - 2>();
+    const Pack<T_, V>*zl = stages + got * STAGE, *hr = zl + P * 32;
+    got = got + 1 == S ? 0 : got + 1;
+    const int live = rows_left<P>(t, len), rows = rows_left<P>(t, end);
+    const bool whole = t + P <= all_len;
+    Vec<V> ga[P], gb[P];
+    Map<V> m;
+    auto gates = [&](auto all) {
+      constexpr bool ALL = decltype(all)::value;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const bool there = ALL || p < live;
+        const Cell<V> k = mingru_cell<V, false>(widen(zl[p * 32], there, -INFINITY),
+                                                widen(hr[p * 32], there, 0.f));
+        ga[p] = k.a;
+        gb[p] = k.b;
+        m = p ? then<V>(m, {k.a, k.b}) : Map<V>{k.a, k.b};
+      }
+    };
+    if (whole) gates(std::true_type{});
+    else gates(std::false_type{});
+    fetch(i + S - 1 < steps);
+    s = exchange<V, false>(K, at, i, m, walk, waiting);
     if (states && rows > 0 && t % kSpan == 0)
 #pragma unroll
-      for (int v = 0; v < V; ++v) states[t / kSpan * chains + at.chain + v] = s[v];
+      for (int v = 0; v < V; ++v) states[t / kSpan * chains + at.chain + v] = s.v[v];
+    auto finish = [&](auto all) {
+      constexpr bool ALL = decltype(all)::value;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      Pack<T_, V> y;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        s[v] = __fmaf_rn(ga[p][v], s[v], gb[p][v]);
-        y.v[v] = from_f32<T_>(p < was ? s[v] : 0.f);
+      for (int p = 0; p < P; ++p) {
+        s = vfma(ga[p], s, gb[p]);
+        if (ALL || p < rows)
+          store_rounded<T_, V>(row_at(o, o_row, p), ALL || p < live ? s : all_of<V>(0.f));
       }
-      if (p < rows) *reinterpret_cast<Pack<T_, V>*>(o + p * hs.row) = y;
-    }
+    };
+    if (whole) finish(std::true_type{});
+    else finish(std::false_type{});
     if (i + 1 < steps) leave<V, false>(K, at, i & 1, s);
     t += step;
-    o += step * hs.row;
+    o += o_step;
   }
   // the state after the last position: the walk's last warp has applied all
   if (h_last && at.in && at.rank == ranks - 1 && at.warp == warps - 1)
 #pragma unroll
-    for (int v = 0; v < V; ++v) h_last[at.chain + v] = s[v];
+    for (int v = 0; v < V; ++v) h_last[at.chain + v] = s.v[v];
+  K.finish();
 }
 
 // ----------------------------------------------------------------- backward
 template <typename T_, int V>
-__global__ void __launch_bounds__(kMaxWarps * 32, V == 1 ? 2 : 1)
-mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains, int warps,
-                   int ranks, const int* __restrict__ lengths, const float* __restrict__ states,
-                   const T_* __restrict__ dh, RowStrides dhs, const float* dh_last, T_* __restrict__ dzh,
-                   RowStrides dzs, float* dh0) {
-  constexpr int P = kGradSteps;
-  __shared__ Walk<V> K;
-  __shared__ Map<V> forward[2][kMaxWarps][32];  // the warps' maps of the state
-  if (ranks > 1) cluster_sync_all();  // the others' shared memory is there from here on
+__global__ void __maxnreg__(kGradRegs)
+mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains,
+                   const int* __restrict__ lengths, const float* __restrict__ states, const T_* __restrict__ dh,
+                   RowStrides dhs, const float* dh_last, T_* __restrict__ dzh, RowStrides dzs, float* dh0, int warps,
+                   int ranks) {
+  constexpr int P = kGradSteps, S = kStages, STAGE = 3 * P * 32;
+  extern __shared__ __align__(16) uint8_t walk_smem[];
+  const Walk<V> K(walk_smem, ranks, true);
+  K.start();
   const Place at = place_of<V>(warps, ranks, chains, d, by_d);
   int len = at.in ? T : 0;
   if (at.in && lengths) len = min(max(lengths[at.b], 0), T);
+  const int end = at.in ? T : 0;
+  const int all_len = __reduce_min_sync(~0u, len);  // positions that all of the warp's chains have
   const int step = ranks * warps * P;
   const int steps = (T + step - 1) / step;
-  long long t = (long long)(steps - 1) * step + (at.rank * warps + at.warp) * P;
-  // the saved state that this warp's positions follow, and the warps between
-  const int since = min(warps, kSpan / P), lead = at.warp % since;
+  // steps are taken from the last
+  int t = (steps - 1) * step + (at.rank * warps + at.warp) * P;
+  // the warps between the saved state and this warp's positions
+  const int lead = at.warp % min(warps, kSpan / P);
   const T_* x = zh + at.b * zs.chunk + t * zs.row + at.c;
   const T_* u = dh + at.b * dhs.chunk + t * dhs.row + at.c;
   T_* o = dzh + at.b * dzs.chunk + t * dzs.row + at.c;
-  Pack<T_, V> zl[P], hr[P], du[P];
-  float saved[V];
-  auto count = [&](int end, long long from) { return (int)max(min((long long)P, end - from), 0ll); };
-  auto load_all = [&](int n) {
-    load_rows(zl, x, zs.row, n, -INFINITY);
-    load_rows(hr, x + d, zs.row, n, 0.f);
-    load_rows(du, u, dhs.row, n, 0.f);
-    const long long k = t / kSpan;
-#pragma unroll
-    for (int v = 0; v < V; ++v) saved[v] = n > 0 ? states[k * chains + at.chain + v] : 0.f;
+  const long long x_step = step * zs.row, u_step = step * dhs.row, o_step = step * dzs.row;
+  const uint32_t x_row = (uint32_t)(zs.row * sizeof(T_)), u_row = (uint32_t)(dhs.row * sizeof(T_)),
+                 o_row = (uint32_t)(dzs.row * sizeof(T_));
+  Vec<V> next_saved = all_of<V>(0.f);  // the saved state of the step after the current one
+  Pack<T_, V>* const stages = warp_stages<T_, V, P, 3>(K.stages, S);
+  int t_next = t, put = 0, got = 0;  // the next step to fetch, its stage, and the stage in use
+  auto fetch = [&](bool more) {
+    if (more) {
+      const int live = rows_left<P>(t_next, len);
+      const bool whole = t_next + P <= all_len;
+      copy_rows<P>(stages + put * STAGE, x, x_row, live, whole);
+      copy_rows<P>(stages + put * STAGE + P * 32, x + d, x_row, live, whole);
+      copy_rows<P>(stages + put * STAGE + 2 * P * 32, u, u_row, live, whole);
+      x -= x_step;
+      u -= u_step;
+      t_next -= step;
+      put = put + 1 == S ? 0 : put + 1;
+    }
+    copies_commit();
   };
-  int live = count(len, t);
-  load_all(live);
-  float s[V], g[V], walk[V];
+  auto load_saved = [&](int from) {
+    if (from < len)
 #pragma unroll
-  for (int v = 0; v < V; ++v) walk[v] = at.in && dh_last ? dh_last[at.chain + v] : 0.f;
+      for (int v = 0; v < V; ++v) next_saved.v[v] = states[from / kSpan * chains + at.chain + v];
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch(i < steps);
+  load_saved(t);
+  Vec<V> walk = all_of<V>(0.f), g = walk;
+  bool waiting = true;
+  if (at.in && dh_last)
+#pragma unroll
+    for (int v = 0; v < V; ++v) walk.v[v] = dh_last[at.chain + v];
   for (int i = 0; i < steps; ++i) {
-    // c carries its branch in its sign: c >= 0, and a negative hr makes it -c
-    float ga[P][V], gz[P][V], gc[P][V], gu[P][V];
-    Map<V> m = identity_map<V>(), r = identity_map<V>();
+    copies_wait<S - 2>();
+    const Pack<T_, V>*zl = stages + got * STAGE, *hr = zl + P * 32, *du = hr + P * 32;
+    got = got + 1 == S ? 0 : got + 1;
+    const int live = rows_left<P>(t, len), rows = rows_left<P>(t, end);
+    Vec<V> s = next_saved;
+    if (i + 1 < steps) load_saved(t - step);
+    const bool whole = t + P <= all_len;
+    Vec<V> ga[P], gb[P], gz[P], gw[P];
+    Map<V> m, r;
+    auto gates = [&](auto all) {
+      constexpr bool ALL = decltype(all)::value;
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float raw = to_f32(hr[p].v[v]);
-        const Cell k = mingru_cell(to_f32(zl[p].v[v]), raw);
-        ga[p][v] = k.a;
-        gz[p][v] = k.z;
-        gc[p][v] = copysignf(k.c, raw);
-        gu[p][v] = to_f32(du[p].v[v]);
-        m.B[v] = __fmaf_rn(k.a, m.B[v], k.z * k.c);
-        m.A[v] *= k.a;
+      for (int p = 0; p < P; ++p) {
+        const bool there = ALL || p < live;
+        const Cell<V> k = mingru_cell<V, true>(widen(zl[p * 32], there, -INFINITY),
+                                               widen(hr[p * 32], there, 0.f));
+        ga[p] = k.a;
+        gb[p] = k.b;
+        gz[p] = k.z;
+        gw[p] = k.w;
+        m = p ? then<V>(m, {k.a, k.b}) : Map<V>{k.a, k.b};
       }
+    };
+    if (whole) gates(std::true_type{});
+    else gates(std::false_type{});
+    // the gradient that reaches each state: G_p = u_p + a_{p+1} G_{p+1}
+    r.A = m.A;
+    r.B = widen(du[(P - 1) * 32], P - 1 < live, 0.f);
 #pragma unroll
-    for (int p = P - 1; p >= 0; --p)
+    for (int p = P - 2; p >= 0; --p) r.B = vfma(ga[p + 1], r.B, widen(du[p * 32], p < live, 0.f));
+    r.B = vmul(ga[0], r.B);
+    fetch(i + S - 1 < steps);
+    Map<V>* forward = K.forward + ((i & 1) * K.warps + at.first) * 32 + at.lane;
+    forward[at.warp * 32] = m;
+    g = exchange<V, true>(K, at, i, r, walk, waiting);
+#pragma unroll 4
+    for (int w = at.warp - lead; w < at.warp; ++w) s = apply<V>(forward[w * 32], s);
+    // dzl / G = a (z c - z h'), h' the state before
 #pragma unroll
-      for (int v = 0; v < V; ++v) r.B[v] = ga[p][v] * (r.B[v] + gu[p][v]);
+    for (int p = 0; p < P; ++p) {
+      Vec<V> gap;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      r.A[v] = m.A[v];
-      s[v] = saved[v];
+      for (int v = 0; v < V; ++v) gap.v[v] = __fmaf_rn(-gz[p].v[v], s.v[v], gb[p].v[v]);
+      gz[p] = vmul(ga[p], gap);
+      s = vfma(ga[p], s, gb[p]);
     }
-    const int rows = at.in ? count(T, t) : 0, was = live;
-    if (i + 1 < steps) {
-      x -= step * zs.row;
-      u -= step * dhs.row;
-      t -= step;
-      live = count(len, t);
-      load_all(live);
-    }
-    forward[i & 1][at.first + at.warp][at.lane] = m;
-    exchange<V, true>(K, at, i & 1, r, walk, g, i == 0);
-    for (int w = at.warp - lead; w < at.warp; ++w) apply<V>(forward[i & 1][at.first + w][at.lane], s);
-    float before[P][V];
+    auto finish = [&](auto all) {
+      constexpr bool ALL = decltype(all)::value;
 #pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        before[p][v] = s[v];
-        s[v] = __fmaf_rn(ga[p][v], s[v], gz[p][v] * fabsf(gc[p][v]));
+      for (int p = P - 1; p >= 0; --p) {
+        const bool there = ALL || p < live;
+        const Vec<V> u_p = widen(du[p * 32], there, 0.f);
+        g = vfma(p == P - 1 ? all_of<V>(1.f) : ga[p + 1], g, u_p);
+        if (ALL || p < rows) {
+          T_* y = row_at(o, o_row, p);
+          store_rounded<T_, V>(y, there ? vmul(g, gz[p]) : all_of<V>(0.f));
+          store_rounded<T_, V>(y + d, there ? vmul(g, gw[p]) : all_of<V>(0.f));
+        }
       }
-#pragma unroll
-    for (int p = P - 1; p >= 0; --p) {
-      Pack<T_, V> yz, yr;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float k = fabsf(gc[p][v]);
-        g[v] += gu[p][v];
-        const float z = g[v] * gz[p][v];
-        const float dz = z * ga[p][v] * (k - before[p][v]);
-        const float dr = signbit(gc[p][v]) ? z * (k - k * k) : z;
-        g[v] *= ga[p][v];
-        yz.v[v] = from_f32<T_>(p < was ? dz : 0.f);
-        yr.v[v] = from_f32<T_>(p < was ? dr : 0.f);
-      }
-      if (p < rows) {
-        *reinterpret_cast<Pack<T_, V>*>(o + p * dzs.row) = yz;
-        *reinterpret_cast<Pack<T_, V>*>(o + p * dzs.row + d) = yr;
-      }
-    }
+      g = vmul(g, ga[0]);
+    };
+    if (whole) finish(std::true_type{});
+    else finish(std::false_type{});
     if (i + 1 < steps) leave<V, true>(K, at, i & 1, g);
-    o -= step * dzs.row;
+    t -= step;
+    o -= o_step;
   }
   if (dh0 && at.in && at.rank == 0 && at.warp == 0)
 #pragma unroll
-    for (int v = 0; v < V; ++v) dh0[at.chain + v] = g[v];
+    for (int v = 0; v < V; ++v) dh0[at.chain + v] = g.v[v];
+  K.finish();
 }
 
 // ------------------------------------------------------------- few positions
-// Up to kScanSteps positions (the decode step): a thread takes V chains through
+// Up to kFew positions (the decode step): a thread takes V chains through
 // all of them, all loads issued first.
 template <typename T_, int V, int STEPS>
 __global__ void __launch_bounds__(256)
@@ -421,31 +665,26 @@ mingru_step_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
       zl[p] = *reinterpret_cast<const Pack<T_, V>*>(x + p * zs.row);
       hr[p] = *reinterpret_cast<const Pack<T_, V>*>(x + p * zs.row + d);
     }
-  float s[V];
+  Vec<V> s;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    s[v] = h0 ? h0[chain + v] : 0.f;
-    if (states && T > 0) states[chain + v] = s[v];
+    s.v[v] = h0 ? h0[chain + v] : 0.f;
+    if (states && T > 0) states[chain + v] = s.v[v];
   }
   T_* o = h + b * hs.chunk + c;
 #pragma unroll
   for (int p = 0; p < STEPS; ++p) {
     if (p >= T) break;
-    Pack<T_, V> y;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      y.v[v] = from_f32<T_>(0.f);
-      if (p < len) {
-        const Cell k = mingru_cell(to_f32(zl[p].v[v]), to_f32(hr[p].v[v]));
-        s[v] = k.a * s[v] + k.z * k.c;
-        y.v[v] = from_f32<T_>(s[v]);
-      }
+    Vec<V> y = all_of<V>(0.f);
+    if (p < len) {
+      const Cell<V> k = mingru_cell<V, false>(widen(zl[p], true, 0.f), widen(hr[p], true, 0.f));
+      y = s = vfma(k.a, s, k.b);
     }
-    *reinterpret_cast<Pack<T_, V>*>(o + p * hs.row) = y;
+    store_rounded<T_, V>(o + p * hs.row, y);
   }
   if (h_last)
 #pragma unroll
-    for (int v = 0; v < V; ++v) h_last[chain + v] = s[v];
+    for (int v = 0; v < V; ++v) h_last[chain + v] = s.v[v];
 }
 
 // ------------------------------------------------------------------ launches
@@ -457,26 +696,62 @@ static bool pairs_ok(int d, int type, std::initializer_list<std::pair<const void
   return true;
 }
 
-// The shape of a walk over `groups` groups of T positions, P to a warp.
+// The shape of a walk: warps of a group in a block, blocks of a group, groups
+// of a block.
 struct Shape {
-  int warps, ranks;     // warps of a group in a block, blocks of a group
-  unsigned blocks, threads;
+  int warps, ranks, per;
 };
-static Shape shape_of(long long groups, int T, int P) {
-  Shape s{1, 1, 0, 0};
-  const int block_warps = groups < 300 ? kMaxWarps : kMaxWarps / 2;
-  while (s.warps < block_warps && (long long)s.warps * P < T) s.warps *= 2;
-  const int per = (long long)s.warps * P >= T ? block_warps / s.warps : 1;  // groups of a block
-  while (s.ranks < kMaxCluster && groups * s.ranks * 2 <= 148 && (long long)s.ranks * s.warps * P < T) s.ranks *= 2;
-  s.blocks = (unsigned)((groups + per - 1) / per * s.ranks);
-  s.threads = (unsigned)(s.warps * per * 32);
-  return s;
-}
-template <typename K, typename... A>
-static cudaError_t launch_walk(K kernel, const Shape& s, cudaStream_t st, A... args) {
+// Clusters of `ranks` blocks that the device holds at once.
+template <typename K>
+static int clusters_at_once(K kernel, int ranks, unsigned threads, size_t smem) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(s.blocks);
-  cfg.blockDim = dim3(s.threads);
+  cfg.gridDim = dim3((unsigned)ranks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return n;
+}
+// Launches `kernel` over `chains` chains of T positions, P to a warp;
+// smem(warps, ranks) gives a block's shared memory.
+template <int V, typename K, typename M, typename... A>
+static cudaError_t launch_walk(K kernel, long long chains, int T, int P, M smem, cudaStream_t st, A... args) {
+  const long long groups = (chains + 32 * V - 1) / (32 * V);
+  Shape s{1, 1, 1};
+  const bool dense = groups >= 148;  // enough groups to give every SM blocks of its own
+  const int block_warps = dense ? kMaxWarps / 2 : kMaxWarps;
+  while (s.warps < block_warps && (long long)s.warps * P < T) s.warps *= 2;
+  if (s.warps > block_warps) s.warps = block_warps;
+  if ((long long)s.warps * P >= T) s.per = block_warps / s.warps;
+  const unsigned threads = (unsigned)(s.warps * s.per * 32);
+  size_t bytes = smem((int)threads / 32, kMaxCluster);
+  // clusters are packed: two of their blocks on one SM while another stays
+  // empty, unless a block takes more than half of the shared memory
+  const size_t alone = bytes < 116 * 1024 ? 116 * 1024 : bytes;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)alone);
+  if (e != cudaSuccess) return e;
+  if (s.per == 1 && groups * 2 <= 148) {
+    int most = kMaxCluster;
+    while (most > 1 && (long long)(most - 1) * s.warps * P >= T) --most;
+    for (int r = most; r > 1; --r)
+      if (groups * r <= 148 && clusters_at_once(kernel, r, threads, alone) >= groups) {
+        s.ranks = r;
+        break;
+      }
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((groups + s.per - 1) / s.per * s.ranks));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = s.ranks > 1 && !dense ? alone : smem((int)threads / 32, s.ranks);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -484,7 +759,7 @@ static cudaError_t launch_walk(K kernel, const Shape& s, cudaStream_t st, A... a
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = s.ranks > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  e = cudaLaunchKernelEx(&cfg, kernel, args..., s.warps, s.ranks);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -500,21 +775,23 @@ cudaError_t launch_mingru_scan(const void* zh, int type, RowStrides zs, int B, i
     E* o = static_cast<E*>(h);
     auto go = [&](auto vec) -> cudaError_t {
       constexpr int V = decltype(vec)::value;
-      if (T <= kScanSteps) {
+      if (T <= kFew) {
         const unsigned blocks = (unsigned)((chains + 256 * V - 1) / (256 * V));
         if (T <= 1)
           mingru_step_kernel<E, V, 1><<<blocks, 256, 0, st>>>(x, zs, T, d, by_d, chains, lengths, h0, o, hs, h_last,
                                                               states);
         else
-          mingru_step_kernel<E, V, kScanSteps><<<blocks, 256, 0, st>>>(x, zs, T, d, by_d, chains, lengths, h0, o, hs,
+          mingru_step_kernel<E, V, kFew><<<blocks, 256, 0, st>>>(x, zs, T, d, by_d, chains, lengths, h0, o, hs,
                                                                        h_last, states);
         return cudaGetLastError();
       }
-      const Shape s = shape_of((chains + 32 * V - 1) / (32 * V), T, kScanSteps);
-      return launch_walk(mingru_scan_kernel<E, V>, s, st, x, zs, T, d, by_d, chains, s.warps, s.ranks, lengths, h0, o,
-                         hs, h_last, states);
+      auto smem = [](int w, int ranks) {
+        return Walk<V>::bytes(w, ranks, false) + (size_t)kStages * 2 * scan_steps<E, V>() * w * 32 * sizeof(Pack<E, V>);
+      };
+      return launch_walk<V>(mingru_scan_kernel<E, V>, chains, T, scan_steps<E, V>(), smem, st, x, zs, T, d, by_d, chains,
+                            lengths, h0, o, hs, h_last, states);
     };
-    return pairs && (sizeof(E) == 2 || T <= kScanSteps) ? go(std::integral_constant<int, 2>{})
+    return pairs && (sizeof(E) == 2 || T <= kFew || chains >= 148 * 64) ? go(std::integral_constant<int, 2>{})
                                                         : go(std::integral_constant<int, 1>{});
   });
 }
@@ -534,10 +811,12 @@ cudaError_t launch_mingru_scan_grad(const void* zh, int type, RowStrides zs, int
     using E = decltype(t);
     auto go = [&](auto vec) {
       constexpr int V = decltype(vec)::value;
-      const Shape s = shape_of((chains + 32 * V - 1) / (32 * V), T, kGradSteps);
-      return launch_walk(mingru_grad_kernel<E, V>, s, st, static_cast<const E*>(zh), zs, T, d, by_d, chains, s.warps,
-                         s.ranks, lengths, states, static_cast<const E*>(dh), dhs, dh_last, static_cast<E*>(dzh), dzs,
-                         dh0);
+      auto smem = [](int w, int ranks) {
+        return Walk<V>::bytes(w, ranks, true) + (size_t)kStages * 3 * kGradSteps * w * 32 * sizeof(Pack<E, V>);
+      };
+      return launch_walk<V>(mingru_grad_kernel<E, V>, chains, T, kGradSteps, smem, st, static_cast<const E*>(zh), zs,
+                            T, d, by_d, chains, lengths, states, static_cast<const E*>(dh), dhs, dh_last,
+                            static_cast<E*>(dzh), dzs, dh0);
     };
     return pairs && sizeof(E) == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
   });

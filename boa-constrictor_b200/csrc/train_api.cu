@@ -29,15 +29,15 @@ bool elem_aligned(const void* p, int type) { return boa::aligned_to(p, boa::type
 bool token_aligned(const void* p, int t) {
   return boa::aligned_to(p, t == BOA_TOK_U8 ? 1 : t == BOA_TOK_I32 ? 4 : 8);
 }
-// b * chunk + t * row + width stays within 63 bits.  Rows that are read may
+// Rows are below 4 GiB apart, and b * chunk stays within 63 bits.  Rows that are read may
 // coincide (an expanded gradient has strides of 0); rows that are written may
 // not, with the chunks outside the positions or inside.
-bool in_strides_ok(int64_t row, int64_t chunk, int B, int T) {
-  const int64_t lim = (int64_t)1 << 60;
-  return row >= 0 && chunk >= 0 && row <= lim / (T + 1ll) && chunk <= lim / (B + 1ll);
+bool in_strides_ok(int64_t row, int64_t chunk, int B, int T, int type) {
+  return row >= 0 && row < (1ll << 40) && (T <= 1 || row * boa::type_bytes(type) <= 0xffffffffll) && chunk >= 0 &&
+         chunk <= ((int64_t)1 << 60) / (B + 1ll);
 }
-bool out_strides_ok(int64_t row, int64_t chunk, int B, int T, int width) {
-  if (!in_strides_ok(row, chunk, B, T)) return false;
+bool out_strides_ok(int64_t row, int64_t chunk, int B, int T, int width, int type) {
+  if (!in_strides_ok(row, chunk, B, T, type)) return false;
   if (B <= 1 || T <= 1) return (T <= 1 || row >= width) && (B <= 1 || chunk >= width);
   return (row >= width && chunk >= (T - 1) * row + width) || (chunk >= width && row >= (B - 1) * chunk + width);
 }
@@ -103,10 +103,11 @@ int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk
                     const int32_t* d_lengths, const float* d_h0, void* d_h, int64_t h_row, int64_t h_chunk,
                     float* d_h_last, float* d_states, void* stream) {
   BOA_REQUIRE(type_ok(type), "unknown element type");
-  BOA_REQUIRE(n_chunks >= 0 && T >= 0, "negative size");
+  BOA_REQUIRE(n_chunks >= 0 && T >= 0 && T <= 1 << 30, "n_chunks must not be negative, T must be 0 .. 2^30");
   BOA_REQUIRE(d >= 1 && d <= boa::kMaxWidth, "d must be 1 .. 65536");
   BOA_REQUIRE((int64_t)n_chunks * d <= 0x7fffffff, "n_chunks * d must be at most 2^31 - 1");
-  BOA_REQUIRE(in_strides_ok(zh_row, zh_chunk, n_chunks, T) && out_strides_ok(h_row, h_chunk, n_chunks, T, d),
+  BOA_REQUIRE(in_strides_ok(zh_row, zh_chunk, n_chunks, T, type) &&
+                  out_strides_ok(h_row, h_chunk, n_chunks, T, d, type),
               "a stride is negative or too large, or the rows of h overlap");
   if (n_chunks == 0) return BOA_OK;
   BOA_REQUIRE(T == 0 || (d_zh && d_h), "null buffer");
@@ -123,11 +124,12 @@ int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t
                              int64_t dh_chunk, const float* d_dh_last, void* d_dzh, int64_t dzh_row,
                              int64_t dzh_chunk, float* d_dh0, void* stream) {
   BOA_REQUIRE(type_ok(type), "unknown element type");
-  BOA_REQUIRE(n_chunks >= 0 && T >= 0, "negative size");
+  BOA_REQUIRE(n_chunks >= 0 && T >= 0 && T <= 1 << 30, "n_chunks must not be negative, T must be 0 .. 2^30");
   BOA_REQUIRE(d >= 1 && d <= boa::kMaxWidth, "d must be 1 .. 65536");
   BOA_REQUIRE((int64_t)n_chunks * d <= 0x7fffffff, "n_chunks * d must be at most 2^31 - 1");
-  BOA_REQUIRE(in_strides_ok(zh_row, zh_chunk, n_chunks, T) && in_strides_ok(dh_row, dh_chunk, n_chunks, T) &&
-                  out_strides_ok(dzh_row, dzh_chunk, n_chunks, T, 2 * d),
+  BOA_REQUIRE(in_strides_ok(zh_row, zh_chunk, n_chunks, T, type) &&
+                  in_strides_ok(dh_row, dh_chunk, n_chunks, T, type) &&
+                  out_strides_ok(dzh_row, dzh_chunk, n_chunks, T, 2 * d, type),
               "a stride is negative or too large, or the rows of dzh overlap");
   if (n_chunks == 0) return BOA_OK;
   BOA_REQUIRE(T == 0 || (d_zh && d_states && d_dh && d_dzh), "null buffer");

@@ -284,6 +284,8 @@ int boa_embed_backward(const void* d_tokens, int token_type, int64_t n, const vo
 /* The minGRU recurrence (BOA_BACKBONE_MINGRU's cell) over T positions of
  * n_chunks chunks.  Position t of chunk b is the row of 2d elements at
  * zh + b * zh_chunk + t * zh_row: d gate logits zl, then d candidates hr.
+ * Strides are in elements; T <= 2^30 and rows lie less than 4 GiB apart.
+ * Inputs may have strides of 0; rows that are written may not overlap.
  *   z = sigmoid(zl); c = hr >= 0 ? hr + 1/2 : sigmoid(hr)
  *   h[b][t] = (1 - z) h[b][t-1] + z c
  * d_lengths (NULL = all T) gives each chunk's positions, clamped to 0 .. T:

@@ -302,16 +302,23 @@ def test_mingru_takes_an_expanded_gradient(tr):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
-def test_mingru_writes_only_its_rows(tr):
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,T,d", [(3, 200, 24), (1, 1200, 160), (9, 515, 160), (3, 900, 64), (40, 77, 33), (2, 2049, 32),
+                                   (200, 97, 96), (200, 300, 64)])
+def test_mingru_writes_only_its_rows(tr, dtype, B, T, d):
+    """Sequences that end inside a step of the kernels' walk: what lies before,
+    behind and beside the rows is left alone."""
     import torch
-    zh, h0, n, dh, dl = _case(torch, np.random.default_rng(10), 3, 200, 24, "bfloat16", [200, 50, 0])
-    out = torch.full((3, 205, 30), 7.0, dtype=torch.bfloat16, device="cuda")
-    _, _, states = tr.mingru_scan(zh, h0, n, out=out[:, 2:202, 3:27], save_states=True)
-    grad = torch.full((3, 205, 50), 7.0, dtype=torch.bfloat16, device="cuda")
-    tr.mingru_scan_backward(zh, states, dh, dl, n, out=grad[:, 2:202, 1:49])
-    for x, lo, hi in ((out, 3, 27), (grad, 1, 49)):
-        assert not (x[:, 2:202, lo:hi] == 7.0).all(-1).any()
-        x[:, 2:202, lo:hi] = 7.0
+    lengths = [T, T // 2, 0, T - 1][:B] + [T] * (B - 4)
+    zh, h0, n, dh, dl = _case(torch, np.random.default_rng(10), B, T, d, dtype, lengths)
+    margin = 600  # rows; more than a step of the walk may reach beyond the end
+    out = torch.full((B, T + 2 * margin, d + 6), 7.0, dtype=zh.dtype, device="cuda")
+    _, _, states = tr.mingru_scan(zh, h0, n, out=out[:, margin:margin + T, 3:3 + d], save_states=True)
+    grad = torch.full((B, T + 2 * margin, 2 * d + 2), 7.0, dtype=zh.dtype, device="cuda")
+    tr.mingru_scan_backward(zh, states, dh, dl, n, out=grad[:, margin:margin + T, 1:1 + 2 * d])
+    for x, lo, hi in ((out, 3, 3 + d), (grad, 1, 1 + 2 * d)):
+        assert not (x[:, margin:margin + T, lo:hi] == 7.0).all(-1).any()
+        x[:, margin:margin + T, lo:hi] = 7.0
         assert (x == 7.0).all()
 
 
@@ -472,12 +479,11 @@ def test_offsets_past_32_bits(tr):
     got = tr.embed_backward(tok, out, 256)
     ref, err = R.embed_grad(_n(tok[-1000:]).astype(np.int64), _n(out[-1000:]), 256, 1.0)
     _close(got[:200], ref[:200], err[:200], "float32")
-    # chunks, and positions, further apart than 2^31 elements
-    zh, h0, _, dh, dl = _case(torch, np.random.default_rng(1), 2, 2, 256, "bfloat16")
+    # chunks further apart than 2^31 elements, and positions almost 2^32 bytes
     far = out.view(-1)
-    step = (1 << 31) + 8
-    for where in ((step, 512), (512, step)):
-        v = far.as_strided((2, 2, 512), (*where, 1))
+    for T, where in ((16, ((1 << 31) + 8, 512)), (2, (512, (1 << 31) - 8))):
+        zh, h0, _, dh, dl = _case(torch, np.random.default_rng(1), 2, T, 256, "bfloat16")
+        v = far.as_strided((2, T, 512), (*where, 1))
         v.copy_(zh)
         h, last, states = tr.mingru_scan(v, h0, save_states=True)
         a = tr.mingru_scan(zh, h0, save_states=True)

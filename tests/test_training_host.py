@@ -46,7 +46,7 @@ REFUSED = [
     (_embed_bwd, dict(p=(A, A, None, A))), (_embed_bwd, dict(p=(A, A, A, None))),
     (_embed_bwd, dict(p=(A, A, A, C.c_void_p(264)))), (_embed_bwd, dict(ws=64)), (_embed_bwd, dict(n=0, p=(A, A, None, A))),
     (_scan, dict(t=3)), (_scan, dict(B=-1)), (_scan, dict(T=-1)), (_scan, dict(d=0)), (_scan, dict(d=65537)),
-    (_scan, dict(B=1 << 20, d=4096)), (_scan, dict(zr=-1)), (_scan, dict(zc=1 << 60)), (_scan, dict(hr=15)),
+    (_scan, dict(B=1 << 20, d=4096)), (_scan, dict(zr=-1)), (_scan, dict(zc=1 << 60)), (_scan, dict(zr=1 << 30)), (_scan, dict(t=2, zr=1 << 31)), (_scan, dict(T=(1 << 30) + 1)), (_scan, dict(hr=15)),
     (_scan, dict(hc=150)), (_scan, dict(zh=None)), (_scan, dict(h=None)), (_scan, dict(zh=odd)),
     (_scan, dict(h0=C.c_void_p(258))),
     (_scan_bwd, dict(t=3)), (_scan_bwd, dict(dr=31)), (_scan_bwd, dict(dc=300)), (_scan_bwd, dict(gr=-16)),

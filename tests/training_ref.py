@@ -67,7 +67,8 @@ def mingru(zh, h0, lengths, dh=None, dlast=None):
     for t in range(T):
         h[t + 1] = a[:, t] * h[t] + z[:, t] * c[:, t]
         size[t + 1] = a[:, t] * size[t] + z[:, t] * np.abs(c[:, t])
-        err[t + 1] = a[:, t] * err[t] + k[:, t] * size[t + 1]
+        # a is formed as 1 - z: its error is that of z, not relative to a
+        err[t + 1] = a[:, t] * err[t] + k[:, t] * (size[t + 1] + z[:, t] * size[t])
     out = np.where(live, h[1:].transpose(1, 0, 2), 0.0)
     got = {"h": (out, np.where(live, err[1:].transpose(1, 0, 2), 0.0)), "last": (h[T], err[T])}
     if dh is None:
@@ -79,13 +80,13 @@ def mingru(zh, h0, lengths, dh=None, dlast=None):
         g = g + np.where(on, dh[:, t], 0.0)
         gs = gs + np.where(on, np.abs(dh[:, t]), 0.0)
         ge = ge + np.where(on, k[:, t] * gs, 0.0)
-        za, cp = z[:, t] * a[:, t], np.where(hr[:, t] >= 0, 1.0, c[:, t] * (1 - c[:, t]))
-        near = ge + 4 * k[:, t] * gs
-        dzh[:, t, :d] = np.where(on, g * za * (c[:, t] - h[t]), 0.0)
-        tol[:, t, :d] = np.where(on, za * ((np.abs(c[:, t]) + size[t]) * near + gs * err[t]), 0.0)
-        dzh[:, t, d:] = np.where(on, g * z[:, t] * cp, 0.0)
-        tol[:, t, d:] = np.where(on, z[:, t] * cp * near, 0.0)
-        g, gs, ge = a[:, t] * g, a[:, t] * gs, a[:, t] * ge + k[:, t] * a[:, t] * gs
+        cp = np.where(hr[:, t] >= 0, 1.0, c[:, t] * (1 - c[:, t]))
+        near, zt, at = ge + 4 * k[:, t] * gs, z[:, t], a[:, t]
+        dzh[:, t, :d] = np.where(on, g * zt * at * (c[:, t] - h[t]), 0.0)
+        tol[:, t, :d] = np.where(on, zt * ((np.abs(c[:, t]) + size[t]) * (at * near + k[:, t] * gs) + at * gs * err[t]), 0.0)
+        dzh[:, t, d:] = np.where(on, g * zt * cp, 0.0)
+        tol[:, t, d:] = np.where(on, zt * cp * near, 0.0)
+        g, gs, ge = at * g, at * gs, at * ge + k[:, t] * (at + np.where(on, zt, 0.0)) * gs
     return {**got, "dzh": (dzh, tol), "dh0": (g, ge)}
 
 
