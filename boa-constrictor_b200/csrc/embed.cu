@@ -2,17 +2,20 @@
 //
 //   out[i] = s * E[t_i]          dE[v] = s * sum_{i : t_i = v} dout[i]
 //
-// Forward.  n * d elements leave, and the table (at most 1024 rows) is read
-// from the caches, so the stores set the pace.
+// Lookup.  n * d elements leave, and the table (at most 1024 rows) is read
+// from the caches, so the stores set the pace.  Where there are many more rows
+// than the table has, a block keeps a slice of the table's columns in shared
+// memory, scaled and rounded, and every row leaves by one bulk copy.
 //
 // Gradient.  Every row of dout is read once, whatever its token: the
 // positions are first ordered by token with a stable counting sort (at most
 // 1024 tokens, so one pass), and the sums then run over consecutive sorted
 // positions in registers.  The sorted positions of a token are cut into
-// pieces of equal length, so that a token that makes up most of the input
-// (the zero byte of binary records) is summed by as many blocks as its share
-// of the rows; the pieces' sums are added in order.  Nothing is added
-// atomically in floating point, and the same input gives the same bits.
+// pieces, so that a token that makes up most of the input (the zero byte of
+// binary records) is summed by as many blocks as its share of the rows; the
+// block that finishes a token last adds its pieces' sums in their order.
+// Nothing is added atomically in floating point, and the same input gives the
+// same bits.
 #include "kernels.cuh"
 #include "ptx.cuh"
 #include "train_ops.cuh"
@@ -75,6 +78,58 @@ static cudaError_t embed_run(const Tok* tok, long long n, const TI* table, long 
   return cudaGetLastError();
 }
 
+// Many rows: block (slice, part) holds columns [c0, c0 + cols) of the table in
+// shared memory as they will be stored, with a row of zeros behind them for
+// padding, and sends one bulk copy per row.  The rows of a part go round the
+// warps 32 at a time.
+template <typename Tok, typename TI, typename TO>
+__global__ void __launch_bounds__(kEmbedThreads)
+embed_rows_kernel(const Tok* __restrict__ tok, long long n, const TI* __restrict__ table, long long ld_table,
+                  int vocab, int d, int cols, int slices, float scale, TO* __restrict__ out, long long ld_out) {
+  extern __shared__ __align__(128) uint8_t embed_smem[];
+  TO* rows = reinterpret_cast<TO*>(embed_smem);
+  const int slice = blockIdx.x % slices, part = blockIdx.x / slices, parts = gridDim.x / slices;
+  const int c0 = slice * cols, here = min(cols, d - c0);
+  for (int v = threadIdx.x >> 5; v <= vocab; v += kEmbedThreads / 32)
+    for (int c = threadIdx.x & 31; c < here; c += 32)
+      rows[v * cols + c] = from_f32<TO>(v < vocab ? scale * to_f32(table[v * ld_table + c0 + c]) : 0.f);
+  fence_proxy_async_smem();
+  __syncthreads();
+  const uint32_t bytes = (uint32_t)(here * sizeof(TO));
+  const long long stride = (long long)parts * kEmbedThreads;
+  for (long long i = (long long)part * kEmbedThreads + threadIdx.x; i < n; i += stride) {
+    const int v = token_index(tok[i], vocab);
+    bulk_store(out + i * ld_out + c0, rows + (v < 0 ? vocab : v) * cols, bytes);
+    bulk_commit();
+  }
+  bulk_wait_all();
+}
+constexpr int kEmbedSmem = 200 * 1024;
+// Columns of a slice: 16-byte multiples, so that vocab + 1 rows fit, and as
+// even as can be.  0 where a slice would be under 256 bytes.
+template <typename TO>
+static int embed_slice(int vocab, int d, int& slices) {
+  const int unit = 16 / (int)sizeof(TO), units = d / unit;
+  const int fit = kEmbedSmem / ((vocab + 1) * 16);
+  if (fit < 16 && fit < units) return 0;
+  slices = (units + fit - 1) / fit;
+  const int each = (units + slices - 1) / slices;
+  slices = (units + each - 1) / each;  // none is empty
+  return each * unit;
+}
+template <typename Tok, typename TI, typename TO>
+static cudaError_t embed_rows_run(const Tok* tok, long long n, const TI* table, long long ld_table, int vocab, int d,
+                                  int cols, int slices, float scale, TO* out, long long ld_out, cudaStream_t st) {
+  const size_t smem = (size_t)(vocab + 1) * cols * sizeof(TO);
+  const auto kernel = embed_rows_kernel<Tok, TI, TO>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const int blocks = 148 * (int)(smem <= 110 * 1024 ? 2 : 1) / slices * slices;
+  kernel<<<(unsigned)(blocks < slices ? slices : blocks), kEmbedThreads, smem, st>>>(tok, n, table, ld_table, vocab, d,
+                                                                                    cols, slices, scale, out, ld_out);
+  return cudaGetLastError();
+}
+
 cudaError_t launch_embed(const void* tokens, int tok_t, long long n, const void* table, int table_t,
                          long long ld_table, int vocab, int d, float scale, void* out, int out_t, long long ld_out,
                          cudaStream_t st) {
@@ -90,8 +145,11 @@ cudaError_t launch_embed(const void* tokens, int tok_t, long long n, const void*
         TO* o = static_cast<TO*>(out);
         const bool wide = d % N == 0 && ld_out % N == 0 && ld_table % N == 0 && aligned_to(o, 16) &&
                           aligned_to(e, (int)alignof(Pack<TI, N>));
-        return wide ? embed_run<Tok, TI, TO, N>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st)
-                    : embed_run<Tok, TI, TO, 1>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
+        if (!wide) return embed_run<Tok, TI, TO, 1>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
+        int slices = 1;
+        const int cols = n >= 1024ll * vocab ? embed_slice<TO>(vocab, d, slices) : 0;
+        return cols ? embed_rows_run<Tok, TI, TO>(t, n, e, ld_table, vocab, d, cols, slices, scale, o, ld_out, st)
+                    : embed_run<Tok, TI, TO, N>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
       });
     });
   });
@@ -100,106 +158,103 @@ cudaError_t launch_embed(const void* tokens, int tok_t, long long n, const void*
 // ---------------------------------------------------------------- gradient
 // Workspace, as 32-bit words: counts [V][tiles], then exclusive along the
 // tiles; total [V]; base [V + 1] and piece_base [V + 1], the first sorted
-// position and the first piece of each token; order [n]; and the pieces'
-// sums [pieces][d] in fp32.
+// position and the first piece of each token; done [V], its finished pieces;
+// order [n]; and the pieces' sums [pieces][d] in fp32.
 constexpr int kSortThreads = 256;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kPieceRows = 512;
+constexpr int kSortHeld = 8;                               // tokens that a lane holds at once
+constexpr int kTile = kSortThreads * kSortHeld;            // least tokens of a tile
+constexpr int kMaxTiles = 1024;
 constexpr int kSumThreads = 256;
+constexpr int kSumChunk = 1024;    // positions of a piece in shared memory at once
+constexpr int kMaxPieces = 256;    // of one token: what its last block adds up
+constexpr int kSmallRows = 4096;   // up to here one kernel does all
 
 struct GradPlan {
-  int tiles;           // tiles of the sort
-  int tile;            // tokens per tile, a multiple of 32 * kSortWarps
-  long long pieces;    // most pieces there can be
-  size_t counts, total, base, piece_base, order, part, words;  // offsets in words
+  int tiles, tile;                 // tiles of the sort, tokens of a tile
+  int rows;                        // rows of a piece (more for a token of over kMaxPieces * rows)
+  long long pieces;                // most pieces there can be
+  size_t counts, total, base, piece_base, done, order, part, words;  // offsets in words
 };
-
 static GradPlan grad_plan(long long n, int vocab, int d) {
   GradPlan p{};
-  // at least 4096 tokens a tile, at most about two tiles per SM
-  long long tile = (n + 295) / 296;
-  if (tile < 4096) tile = 4096;
-  tile = (tile + kSortThreads - 1) / kSortThreads * kSortThreads;
+  long long tile = (n + kMaxTiles - 1) / kMaxTiles;
+  tile = (tile + kTile - 1) / kTile * kTile;
   p.tile = (int)tile;
   p.tiles = (int)((n + tile - 1) / tile);
-  p.pieces = n / kPieceRows + vocab;  // sum of ceil(total / kPieceRows)
+  // about eight blocks per SM
+  const long long rows = (n + 148 * 8 - 1) / (148 * 8);
+  p.rows = (int)(rows < 128 ? 128 : (rows + 31) / 32 * 32);
+  p.pieces = n / p.rows + vocab;   // at least the sum of ceil(total / rows)
   auto up4 = [](size_t x) { return (x + 3) & ~(size_t)3; };
   p.counts = 0;
   p.total = up4(p.counts + (size_t)vocab * p.tiles);
   p.base = up4(p.total + vocab);
   p.piece_base = up4(p.base + vocab + 1);
-  p.order = up4(p.piece_base + vocab + 1);
+  p.done = up4(p.piece_base + vocab + 1);
+  p.order = up4(p.done + vocab);
   p.part = up4(p.order + (size_t)n);
   p.words = p.part + (size_t)p.pieces * d;
   return p;
 }
-size_t embed_grad_workspace(long long n, int vocab, int d) { return n > 0 ? grad_plan(n, vocab, d).words * 4 : 0; }
+size_t embed_grad_workspace(long long n, int vocab, int d) {
+  return n > kSmallRows ? grad_plan(n, vocab, d).words * 4 : 0;
+}
+__host__ __device__ inline int rows_of_piece(int total, int rows) {
+  const int most = (total + kMaxPieces - 1) / kMaxPieces;
+  return most > rows ? most : rows;
+}
+__device__ __forceinline__ int pieces_of(int total, int rows) {
+  const int r = rows_of_piece(total, rows);
+  return (total + r - 1) / r;
+}
 
-// Counts of each token in each tile, per warp in shared memory: warp w owns
-// the w-th contiguous part of the tile.  Returns with `mine` complete.
+// The tokens of 32 * kSortHeld positions from `at`, lane by lane; -1 past `end`.
 template <typename Tok>
-__device__ __forceinline__ void count_tile(const Tok* __restrict__ tok, long long w0, long long w1, int vocab,
-                                           int* mine) {
+__device__ __forceinline__ void load_tokens(const Tok* __restrict__ tok, long long at, long long end, int vocab,
+                                            int (&v)[kSortHeld]) {
   const int lane = threadIdx.x & 31;
-  for (long long i = w0 + lane; i < w1; i += 32) {
-    const int v = token_index(tok[i], vocab);
-    if (v >= 0) atomicAdd(mine + v, 1);
+#pragma unroll
+  for (int j = 0; j < kSortHeld; ++j) {
+    const long long i = at + j * 32 + lane;
+    v[j] = i < end ? token_index(tok[i], vocab) : -1;
   }
 }
 
+// Counts of each token in each tile; warp w owns the w-th part of the tile.
 template <typename Tok>
 __global__ void __launch_bounds__(kSortThreads)
 embed_count_kernel(const Tok* __restrict__ tok, long long n, int vocab, int tile, int tiles, int* __restrict__ counts) {
   extern __shared__ int hist[];  // [kSortWarps][vocab]
   const int warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kSortWarps * vocab; i += kSortThreads) hist[i] = 0;
-  __syncthreads();
   const int span = tile / kSortWarps;
   const long long w0 = (long long)blockIdx.x * tile + (long long)warp * span;
   const long long w1 = w0 + span < n ? w0 + span : n;
-  count_tile(tok, w0, w1, vocab, hist + warp * vocab);
+  int v[kSortHeld];
+  load_tokens(tok, w0, w1, vocab, v);
+  for (int i = threadIdx.x; i < kSortWarps * vocab; i += kSortThreads) hist[i] = 0;
   __syncthreads();
-  for (int v = threadIdx.x; v < vocab; v += kSortThreads) {
+  int* mine = hist + warp * vocab;
+  for (long long at = w0; at < w1; at += 32 * kSortHeld) {
+    if (at > w0) load_tokens(tok, at, w1, vocab, v);
+#pragma unroll
+    for (int j = 0; j < kSortHeld; ++j)
+      if (v[j] >= 0) atomicAdd(mine + v[j], 1);
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < vocab; k += kSortThreads) {
     int s = 0;
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) s += hist[w * vocab + v];
-    counts[(size_t)v * tiles + blockIdx.x] = s;
+    for (int w = 0; w < kSortWarps; ++w) s += hist[w * vocab + k];
+    counts[(size_t)k * tiles + blockIdx.x] = s;
   }
 }
 
-// counts of one token -> exclusive prefix along the tiles, and the total
-__global__ void __launch_bounds__(32) embed_prefix_kernel(int* __restrict__ counts, int tiles, int* __restrict__ total) {
-  const int v = blockIdx.x, lane = threadIdx.x;
-  int* c = counts + (size_t)v * tiles;
-  int run = 0;
-  for (int t0 = 0; t0 < tiles; t0 += 32) {
-    const int x = t0 + lane < tiles ? c[t0 + lane] : 0;
-    int s = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(~0u, s, o);
-      if (lane >= o) s += y;
-    }
-    if (t0 + lane < tiles) c[t0 + lane] = run + s - x;
-    run += __shfl_sync(~0u, s, 31);
-  }
-  if (lane == 0) total[v] = run;
-}
-
-// Exclusive prefix over the tokens of f(total[v]), written to out[0..vocab];
-// whole block, vocab <= 4 * kSortThreads.
-template <typename F>
-__device__ __forceinline__ void vocab_prefix(const int* __restrict__ total, int vocab, F f, int* out, int* scratch) {
-  constexpr int PER = kMaxVocab / kSortThreads;
+// Exclusive prefix of one int per thread over the block; scratch [threads / 32].
+template <int THREADS>
+__device__ __forceinline__ int block_prefix(int x, int* scratch, int& sum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x[PER], sum = 0;
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int v = threadIdx.x * PER + k;
-    x[k] = v < vocab ? f(total[v]) : 0;
-    sum += x[k];
-  }
-  int s = sum;
+  int s = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(~0u, s, o);
@@ -207,15 +262,61 @@ __device__ __forceinline__ void vocab_prefix(const int* __restrict__ total, int 
   }
   if (lane == 31) scratch[warp] = s;
   __syncthreads();
-  int before = s - sum;
-  for (int w = 0; w < warp; ++w) before += scratch[w];
+  int before = s - x;
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += scratch[w];
+    sum += scratch[w];
+  }
+  __syncthreads();
+  return before;
+}
+
+// counts of one token -> exclusive prefix along the tiles, and the total
+constexpr int kPrefixThreads = 128;
+__global__ void __launch_bounds__(kPrefixThreads)
+embed_prefix_kernel(int* __restrict__ counts, int tiles, int* __restrict__ total, int* __restrict__ done) {
+  __shared__ int scratch[kPrefixThreads / 32];
+  constexpr int PER = kMaxTiles / kPrefixThreads;
+  int* c = counts + (size_t)blockIdx.x * tiles;
+  int x[PER], sum = 0, all;
+  const int t0 = threadIdx.x * PER;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int v = threadIdx.x * PER + k;
-    if (v <= vocab) out[v] = before;  // out[vocab] = the sum of all
+    x[k] = t0 + k < tiles ? c[t0 + k] : 0;
+    sum += x[k];
+  }
+  int before = block_prefix<kPrefixThreads>(sum, scratch, all);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if (t0 + k < tiles) c[t0 + k] = before;
     before += x[k];
   }
-  if (threadIdx.x == kSortThreads - 1 && kMaxVocab == vocab) out[vocab] = before;
+  if (threadIdx.x == 0) {
+    total[blockIdx.x] = all;
+    done[blockIdx.x] = 0;
+  }
+}
+
+// Exclusive prefix over the tokens of f(total[v]), written to out[0..vocab].
+template <typename F>
+__device__ __forceinline__ void vocab_prefix(const int* __restrict__ total, int vocab, F f, int* out, int* scratch) {
+  constexpr int PER = kMaxVocab / kSortThreads;
+  int x[PER], sum = 0, all;
+  const int v0 = threadIdx.x * PER;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    x[k] = v0 + k < vocab ? f(total[v0 + k]) : 0;
+    sum += x[k];
+  }
+  int before = block_prefix<kSortThreads>(sum, scratch, all);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if (v0 + k < vocab) out[v0 + k] = before;
+    before += x[k];
+  }
+  if (threadIdx.x == 0) out[vocab] = all;
   __syncthreads();
 }
 
@@ -224,172 +325,311 @@ __device__ __forceinline__ void vocab_prefix(const int* __restrict__ total, int 
 // other with a match, so equal tokens keep the order of their positions.
 template <typename Tok>
 __global__ void __launch_bounds__(kSortThreads)
-embed_order_kernel(const Tok* __restrict__ tok, long long n, int vocab, int tile, int tiles,
+embed_order_kernel(const Tok* __restrict__ tok, long long n, int vocab, int tile, int tiles, int rows,
                    const int* __restrict__ counts, const int* __restrict__ total, int* __restrict__ base_out,
                    int* __restrict__ piece_base, int* __restrict__ order) {
   extern __shared__ int hist[];  // [kSortWarps][vocab] next places, base [vocab + 1], scratch [kSortWarps]
   int* base = hist + kSortWarps * vocab;
   int* scratch = base + vocab + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < kSortWarps * vocab; i += kSortThreads) hist[i] = 0;
-  __syncthreads();
   const int span = tile / kSortWarps;
   const long long w0 = (long long)blockIdx.x * tile + (long long)warp * span;
   const long long w1 = w0 + span < n ? w0 + span : n;
-  count_tile(tok, w0, w1, vocab, hist + warp * vocab);
-  if (blockIdx.x == 0) {  // the pieces of each token, for the kernels that follow
-    vocab_prefix(total, vocab, [](int c) { return (c + kPieceRows - 1) / kPieceRows; }, base, scratch);
-    for (int v = threadIdx.x; v <= vocab; v += kSortThreads) piece_base[v] = base[v];
+  int v[kSortHeld];
+  load_tokens(tok, w0, w1, vocab, v);
+  for (int i = threadIdx.x; i < kSortWarps * vocab; i += kSortThreads) hist[i] = 0;
+  __syncthreads();
+  int* next = hist + warp * vocab;
+  for (long long at = w0; at < w1; at += 32 * kSortHeld) {
+    if (at > w0) load_tokens(tok, at, w1, vocab, v);
+#pragma unroll
+    for (int j = 0; j < kSortHeld; ++j)
+      if (v[j] >= 0) atomicAdd(next + v[j], 1);
+  }
+  if (blockIdx.x == 0) {  // the pieces of each token, for the kernel that follows
+    vocab_prefix(total, vocab, [&](int c) { return pieces_of(c, rows); }, base, scratch);
+    for (int k = threadIdx.x; k <= vocab; k += kSortThreads) piece_base[k] = base[k];
     __syncthreads();
   }
   vocab_prefix(total, vocab, [](int c) { return c; }, base, scratch);
   if (blockIdx.x == 0)
-    for (int v = threadIdx.x; v <= vocab; v += kSortThreads) base_out[v] = base[v];
-  for (int v = threadIdx.x; v < vocab; v += kSortThreads) {
-    int at = base[v] + counts[(size_t)v * tiles + blockIdx.x];
+    for (int k = threadIdx.x; k <= vocab; k += kSortThreads) base_out[k] = base[k];
+  for (int k = threadIdx.x; k < vocab; k += kSortThreads) {
+    int at = base[k] + counts[(size_t)k * tiles + blockIdx.x];
 #pragma unroll
     for (int w = 0; w < kSortWarps; ++w) {
-      const int c = hist[w * vocab + v];
-      hist[w * vocab + v] = at;
+      const int c = hist[w * vocab + k];
+      hist[w * vocab + k] = at;
       at += c;
     }
   }
   __syncthreads();
-  int* next = hist + warp * vocab;
-  for (long long i0 = w0; i0 < w1; i0 += 32) {
-    const long long i = i0 + lane;
-    const int v = i < w1 ? token_index(tok[i], vocab) : -1;
-    const unsigned same = __match_any_sync(~0u, v);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    int at = 0;
-    if (v >= 0) at = next[v] + rank;
-    __syncwarp();
-    if (v >= 0 && rank == 0) next[v] = at + __popc(same);
-    __syncwarp();
-    if (v >= 0) order[at] = (int)i;
+  for (long long at = w0; at < w1; at += 32 * kSortHeld) {
+    if (span > 32 * kSortHeld) load_tokens(tok, at, w1, vocab, v);
+#pragma unroll
+    for (int j = 0; j < kSortHeld; ++j) {
+      const unsigned same = __match_any_sync(~0u, v[j]);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      const int to = v[j] >= 0 ? next[v[j]] + rank : 0;
+      __syncwarp();
+      if (v[j] >= 0) {
+        if (rank == 0) next[v[j]] = to + __popc(same);
+        order[to] = (int)(at + j * 32 + lane);
+      }
+      __syncwarp();
+    }
   }
+}
+
+// A pack of a row that is read once.
+template <typename T_, int N>
+__device__ __forceinline__ Pack<T_, N> load_once(const T_* p) {
+  if constexpr (N * sizeof(T_) == 16) {
+    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
+    return *reinterpret_cast<const Pack<T_, N>*>(&w);
+  } else {
+    return *reinterpret_cast<const Pack<T_, N>*>(p);
+  }
+}
+// out (+)= scale * sum of N columns
+template <typename TD, int N>
+__device__ __forceinline__ void store_grad(TD* out, const float (&sum)[N], float scale, int accumulate) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float r = sum[k] * scale;
+    out[k] = from_f32<TD>(accumulate ? r + to_f32(out[k]) : r);
+  }
+}
+// Adds up what the `groups` groups of `per_row` threads hold, N columns a
+// thread, in the order of the groups; the result is group 0's.
+template <int N>
+__device__ __forceinline__ void join_groups(float (&acc)[N], float* s_sum, int g, int groups, int col, int per_row) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) s_sum[k * kSumThreads + threadIdx.x] = acc[k];
+  __syncthreads();
+  if (g == 0)
+    for (int j = 1; j < groups; ++j)
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] += s_sum[k * kSumThreads + j * per_row + col];
+  __syncthreads();
 }
 
 // Sum of one piece: the block's threads form groups of `per_row` threads, one
 // pack of N columns each; group g takes the piece's rows g, g + groups, ...
-template <typename TG, int N>
+// The block that finishes a token's pieces last adds them up; blocks beyond
+// the last piece see to the tokens that do not occur.
+template <typename TG, typename TD, int N>
 __global__ void __launch_bounds__(kSumThreads)
-embed_sum_kernel(const TG* __restrict__ dout, long long ld, int vocab, int d, int per_row,
-                 const int* __restrict__ base, const int* __restrict__ piece_base, const int* __restrict__ order,
-                 float* __restrict__ part) {
-  __shared__ int s_tok, s_order[kPieceRows];
+embed_sum_kernel(const TG* __restrict__ dout, long long ld, int vocab, int d, int per_row, int rows_least,
+                 const int* __restrict__ total, const int* __restrict__ base, const int* __restrict__ piece_base,
+                 const int* __restrict__ order, int* __restrict__ done, float* __restrict__ part, float scale,
+                 int accumulate, TD* dtable, long long ld_dtable) {
+  __shared__ int s_tok, s_last, s_order[kSumChunk], scratch[kSumThreads / 32];
   __shared__ float s_sum[kSumThreads * N];
-  const int p = blockIdx.x;
-  if (p >= piece_base[vocab]) return;
+  const int p = blockIdx.x, pieces_all = piece_base[vocab];
+  if (threadIdx.x == 0) s_tok = -1;
+  __syncthreads();
+  if (p >= pieces_all) {  // the (p - pieces_all)-th token that does not occur
+    if (accumulate) return;
+    constexpr int PER = kMaxVocab / kSumThreads;
+    int none = 0, all;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) none += threadIdx.x * PER + k < vocab && total[threadIdx.x * PER + k] == 0;
+    int at = block_prefix<kSumThreads>(none, scratch, all);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int v = threadIdx.x * PER + k;
+      if (v < vocab && total[v] == 0 && at++ == p - pieces_all) s_tok = v;
+    }
+    __syncthreads();
+    if (s_tok >= 0)
+      for (int c = threadIdx.x; c < d; c += kSumThreads) dtable[s_tok * ld_dtable + c] = from_f32<TD>(0.f);
+    return;
+  }
   for (int v = threadIdx.x; v < vocab; v += kSumThreads)
     if (piece_base[v] <= p && p < piece_base[v + 1]) s_tok = v;
   __syncthreads();
-  const int v = s_tok;
-  const int first = base[v] + (p - piece_base[v]) * kPieceRows;
-  const int rows = min(kPieceRows, base[v + 1] - first);
-  for (int i = threadIdx.x; i < rows; i += kSumThreads) s_order[i] = order[first + i];
-  __syncthreads();
-  const int groups = kSumThreads / per_row;
-  const int g = threadIdx.x / per_row, col = threadIdx.x - g * per_row;
+  const int v = s_tok, count = total[v], first_piece = piece_base[v], pieces = piece_base[v + 1] - first_piece;
+  const int size = rows_of_piece(count, rows_least);
+  const int begin = (p - first_piece) * size, rows = min(size, count - begin);
+  const int* mine = order + base[v] + begin;
+  const int groups = kSumThreads / per_row, g = threadIdx.x / per_row, col = threadIdx.x - g * per_row;
   const int q = d / N;
   for (int c0 = 0; c0 < q; c0 += per_row) {
     const int c = c0 + col;
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    if (g < groups && c < q) {
-      const TG* col_ptr = dout + (size_t)c * N;
+    for (int r0 = 0; r0 < rows; r0 += kSumChunk) {
+      const int here = min(kSumChunk, rows - r0);
+      if (r0 || !c0) {
+        if (r0) __syncthreads();
+        for (int i = threadIdx.x; i < here; i += kSumThreads) s_order[i] = mine[r0 + i];
+        __syncthreads();
+      } else if (rows > kSumChunk) {  // the first chunk again, for the next columns
+        for (int i = threadIdx.x; i < here; i += kSumThreads) s_order[i] = mine[i];
+        __syncthreads();
+      }
+      if (g < groups && c < q) {
+        const TG* x = dout + (size_t)c * N;
 #pragma unroll 8
-      for (int r = g; r < rows; r += groups) {
-        const Pack<TG, N> x = *reinterpret_cast<const Pack<TG, N>*>(col_ptr + s_order[r] * ld);
+        for (int r = g; r < here; r += groups) {
+          const Pack<TG, N> y = load_once<TG, N>(x + s_order[r] * ld);
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += to_f32(x.v[k]);
+          for (int k = 0; k < N; ++k) acc[k] += to_f32(y.v[k]);
+        }
       }
     }
-    if (c0) __syncthreads();
-#pragma unroll
-    for (int k = 0; k < N; ++k) s_sum[k * kSumThreads + threadIdx.x] = acc[k];
-    __syncthreads();
+    join_groups<N>(acc, s_sum, g, groups, col, per_row);
     if (g == 0 && c < q) {
-      for (int j = 1; j < groups; ++j)
+      if (pieces == 1) {
+        store_grad<TD, N>(dtable + v * ld_dtable + c * N, acc, scale, accumulate);
+      } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += s_sum[k * kSumThreads + j * per_row + col];
-#pragma unroll
-      for (int k = 0; k < N; ++k) part[(size_t)p * d + c * N + k] = acc[k];
+        for (int k = 0; k < N; ++k) __stcg(part + (size_t)p * d + c * N + k, acc[k]);
+      }
     }
   }
-}
-
-// dtable[v][c] = scale * the sum of the token's pieces, in order (fp64: one
-// add per 512 rows): eight threads a column take contiguous runs of pieces.
-template <typename TD>
-__global__ void __launch_bounds__(256)
-embed_join_kernel(const float* __restrict__ part, const int* __restrict__ piece_base, int d, float scale,
-                  int accumulate, TD* __restrict__ dtable, long long ld) {
-  __shared__ double s[8][32];
-  const int v = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
-  const int p0 = piece_base ? piece_base[v] : 0, p1 = piece_base ? piece_base[v + 1] : 0;
-  const int run = (p1 - p0 + 7) / 8;
-  const int a = p0 + g * run, b = min(p1, a + run);
-  double sum = 0.0;
-  if (c < d)
-#pragma unroll 8
-    for (int p = a; p < b; ++p) sum += (double)part[(size_t)p * d + c];
-  s[g][threadIdx.x & 31] = sum;
+  if (pieces == 1) return;
+  __threadfence();
   __syncthreads();
-  if (g == 0 && c < d) {
-    for (int j = 1; j < 8; ++j) sum += s[j][threadIdx.x];
-    TD* out = dtable + v * ld + c;
-    float r = (float)(sum * (double)scale);
-    if (accumulate) r += to_f32(*out);
-    *out = from_f32<TD>(r);
+  if (threadIdx.x == 0) s_last = atomicAdd(done + v, 1) == pieces - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  for (int c0 = 0; c0 < q; c0 += per_row) {
+    const int c = c0 + col;
+    float acc[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+    if (g < groups && c < q) {
+      const float* x = part + (size_t)first_piece * d + c * N;
+#pragma unroll 8
+      for (int r = g; r < pieces; r += groups)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += __ldcg(x + (size_t)r * d + k);
+    }
+    join_groups<N>(acc, s_sum, g, groups, col, per_row);
+    if (g == 0 && c < q) store_grad<TD, N>(dtable + v * ld_dtable + c * N, acc, scale, accumulate);
   }
 }
 
-template <typename TG, int N>
-static void sum_run(const TG* dout, long long ld, int vocab, int d, const GradPlan& p, int* w, cudaStream_t st) {
+// Few rows: one kernel.  A block takes `per` tokens and up to 32 packs of
+// columns; it reads all tokens into shared memory, and for each of its own
+// tokens lists the positions in order (a lane keeps the match mask of every
+// 32 positions of its warp's part) and sums their rows.
+template <typename Tok, typename TG, typename TD, int N>
+__global__ void __launch_bounds__(kSumThreads)
+embed_small_kernel(const Tok* __restrict__ tok, int n, const TG* __restrict__ dout, long long ld, int vocab, int d,
+                   int per, float scale, int accumulate, TD* dtable, long long ld_dtable) {
+  static_assert(kSmallRows <= 32 * 32 * (kSumThreads / 32), "a lane holds one mask");
+  __shared__ short s_tok[kSmallRows], s_order[kSmallRows];
+  __shared__ int s_count[kSumThreads / 32];
+  __shared__ float s_sum[kSumThreads * N];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int q = d / N, c0 = blockIdx.y * 32, packs = min(32, q - c0);
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += kSumThreads) s_tok[i] = (short)token_index(tok[i], vocab);
+  __syncthreads();
+  // this warp's part of the positions: whole groups of 32, at most 16 of them
+  const int span = (n + kSumThreads - 1) / kSumThreads * 32, w0 = warp * span, w1 = min(n, w0 + span);
+  const int groups = kSumThreads / packs, g = threadIdx.x / packs, col = threadIdx.x - g * packs;
+  const int v1 = min(vocab, (int)(blockIdx.x + 1) * per);
+  for (int v = blockIdx.x * per; v < v1; ++v) {
+    unsigned mask = 0;
+    for (int j = 0; w0 + j * 32 < w1; ++j) {
+      const int i = w0 + j * 32 + lane;
+      const unsigned m = __ballot_sync(~0u, i < w1 && s_tok[i] == v);
+      if (lane == j) mask = m;
+    }
+    int at = __popc(mask), sum = at;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(~0u, at, o);
+      if (lane >= o) at += y;
+    }
+    if (lane == 31) s_count[warp] = at;
+    at -= sum;
+    __syncthreads();
+    int rows = 0;
+#pragma unroll
+    for (int w = 0; w < kSumThreads / 32; ++w) {
+      if (w < warp) at += s_count[w];
+      rows += s_count[w];
+    }
+    for (; mask; mask &= mask - 1) s_order[at++] = (short)(w0 + lane * 32 + __ffs(mask) - 1);
+    __syncthreads();
+    float acc[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+    if (g < groups) {
+      const TG* x = dout + (size_t)(c0 + col) * N;
+#pragma unroll 8
+      for (int r = g; r < rows; r += groups) {
+        const Pack<TG, N> y = load_once<TG, N>(x + s_order[r] * ld);
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += to_f32(y.v[k]);
+      }
+    }
+    join_groups<N>(acc, s_sum, g, groups, col, packs);
+    if (g == 0 && (rows || !accumulate))
+      store_grad<TD, N>(dtable + v * ld_dtable + (c0 + col) * N, acc, scale, accumulate);
+  }
+}
+
+template <typename TD>
+__global__ void __launch_bounds__(256) embed_zero_kernel(TD* dtable, long long ld, int d) {
+  for (int c = threadIdx.x; c < d; c += 256) dtable[blockIdx.x * ld + c] = from_f32<TD>(0.f);
+}
+
+template <typename Tok, typename TG, typename TD, int N>
+static cudaError_t grad_run(const Tok* tok, long long n, const TG* dout, long long ld, int vocab, int d, float scale,
+                            bool accumulate, TD* dtable, long long ld_dtable, int* w, cudaStream_t st) {
   const int q = d / N;
-  const int per_row = q < kSumThreads ? q : kSumThreads;
-  embed_sum_kernel<TG, N><<<(unsigned)p.pieces, kSumThreads, 0, st>>>(
-      dout, ld, vocab, d, per_row, w + p.base, w + p.piece_base, w + p.order, reinterpret_cast<float*>(w + p.part));
+  if (n <= kSmallRows) {
+    const int per = (vocab + 147) / 148;
+    embed_small_kernel<Tok, TG, TD, N><<<dim3((vocab + per - 1) / per, (q + 31) / 32), kSumThreads, 0, st>>>(
+        tok, (int)n, dout, ld, vocab, d, per, scale, accumulate ? 1 : 0, dtable, ld_dtable);
+    return cudaGetLastError();
+  }
+  const GradPlan p = grad_plan(n, vocab, d);
+  const size_t hist_bytes = (size_t)kSortWarps * vocab * 4;
+  embed_count_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes, st>>>(tok, n, vocab, p.tile, p.tiles, w + p.counts);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  embed_prefix_kernel<<<vocab, kPrefixThreads, 0, st>>>(w + p.counts, p.tiles, w + p.total, w + p.done);
+  embed_order_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes + (vocab + 1 + kSortWarps) * 4, st>>>(
+      tok, n, vocab, p.tile, p.tiles, p.rows, w + p.counts, w + p.total, w + p.base, w + p.piece_base, w + p.order);
+  embed_sum_kernel<TG, TD, N><<<(unsigned)p.pieces, kSumThreads, 0, st>>>(
+      dout, ld, vocab, d, q < kSumThreads ? q : kSumThreads, p.rows, w + p.total, w + p.base, w + p.piece_base,
+      w + p.order, w + p.done, reinterpret_cast<float*>(w + p.part), scale, accumulate ? 1 : 0, dtable, ld_dtable);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_embed_grad(const void* tokens, int tok_t, long long n, const void* dout, int dout_t,
                               long long ld_dout, int vocab, int d, float scale, bool accumulate, void* dtable,
                               int dtable_t, long long ld_dtable, void* ws, cudaStream_t st) {
-  int* w = static_cast<int*>(ws);
-  const GradPlan p = grad_plan(n > 0 ? n : 1, vocab, d);
-  cudaError_t e = cudaSuccess;
-  if (n > 0) {
-    e = with_token(tok_t, [&](auto tk) {
-      using Tok = decltype(tk);
-      const Tok* t = static_cast<const Tok*>(tokens);
-      const size_t hist_bytes = (size_t)kSortWarps * vocab * 4;
-      embed_count_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes, st>>>(t, n, vocab, p.tile, p.tiles, w + p.counts);
-      embed_prefix_kernel<<<vocab, 32, 0, st>>>(w + p.counts, p.tiles, w + p.total);
-      embed_order_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes + (vocab + 1 + kSortWarps) * 4, st>>>(
-          t, n, vocab, p.tile, p.tiles, w + p.counts, w + p.total, w + p.base, w + p.piece_base, w + p.order);
-      return cudaGetLastError();
-    });
-    if (e != cudaSuccess) return e;
-    e = with_type(dout_t, [&](auto tg) {
-      using TG = decltype(tg);
-      constexpr int N = 16 / sizeof(TG);
-      const TG* x = static_cast<const TG*>(dout);
-      if (d % N == 0 && ld_dout % N == 0 && aligned_to(x, 16)) sum_run<TG, N>(x, ld_dout, vocab, d, p, w, st);
-      else sum_run<TG, 1>(x, ld_dout, vocab, d, p, w, st);
-      return cudaGetLastError();
-    });
-    if (e != cudaSuccess) return e;
-  } else if (accumulate) {
-    return cudaSuccess;
-  }
   return with_type(dtable_t, [&](auto td) {
     using TD = decltype(td);
-    embed_join_kernel<TD><<<dim3((d + 31) / 32, vocab), 256, 0, st>>>(
-        n > 0 ? reinterpret_cast<const float*>(w + p.part) : nullptr, n > 0 ? w + p.piece_base : nullptr, d, scale,
-        accumulate ? 1 : 0, static_cast<TD*>(dtable), ld_dtable);
-    return cudaGetLastError();
+    TD* out = static_cast<TD*>(dtable);
+    if (n == 0) {
+      if (accumulate) return cudaSuccess;
+      embed_zero_kernel<TD><<<vocab, 256, 0, st>>>(out, ld_dtable, d);
+      return cudaGetLastError();
+    }
+    return with_type(dout_t, [&](auto tg) {
+      return with_token(tok_t, [&](auto tk) {
+        using TG = decltype(tg);
+        using Tok = decltype(tk);
+        constexpr int N = 16 / sizeof(TG);
+        const TG* x = static_cast<const TG*>(dout);
+        const Tok* t = static_cast<const Tok*>(tokens);
+        int* w = static_cast<int*>(ws);
+        const bool wide = d % N == 0 && ld_dout % N == 0 && aligned_to(x, 16);
+        return wide ? grad_run<Tok, TG, TD, N>(t, n, x, ld_dout, vocab, d, scale, accumulate, out, ld_dtable, w, st)
+                    : grad_run<Tok, TG, TD, 1>(t, n, x, ld_dout, vocab, d, scale, accumulate, out, ld_dtable, w, st);
+      });
+    });
   });
 }
 

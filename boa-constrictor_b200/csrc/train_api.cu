@@ -38,6 +38,7 @@ bool in_strides_ok(int64_t row, int64_t chunk, int B, int T, int type) {
 }
 bool out_strides_ok(int64_t row, int64_t chunk, int B, int T, int width, int type) {
   if (!in_strides_ok(row, chunk, B, T, type)) return false;
+  if (T == 0) return true;
   if (B <= 1 || T <= 1) return (T <= 1 || row >= width) && (B <= 1 || chunk >= width);
   return (row >= width && chunk >= (T - 1) * row + width) || (chunk >= width && row >= (B - 1) * chunk + width);
 }
@@ -85,8 +86,8 @@ int boa_embed_backward(const void* d_tokens, int token_type, int64_t n, const vo
     BOA_REQUIRE(d_tokens && d_dout, "null buffer");
     BOA_REQUIRE(token_aligned(d_tokens, token_type) && elem_aligned(d_dout, dout_type),
                 "a buffer is not aligned to its element");
-    BOA_REQUIRE(d_workspace && boa::aligned_to(d_workspace, 16) &&
-                    workspace_bytes >= boa::embed_grad_workspace(n, vocab, d),
+    const size_t need = boa::embed_grad_workspace(n, vocab, d);
+    BOA_REQUIRE(need == 0 || (d_workspace && boa::aligned_to(d_workspace, 16) && workspace_bytes >= need),
                 "the workspace is null, not aligned to 16 bytes or below boa_embed_backward_workspace");
   }
   return train_launch(__func__,

@@ -14,7 +14,7 @@ def _embed(L, tok_t=0, n=8, tab_t=0, ld_t=16, vocab=256, d=16, out_t=0, ld_o=16,
     return L.boa_embed(p[0], tok_t, n, p[1], tab_t, ld_t, vocab, d, 1.0, p[2], out_t, ld_o, None)
 
 
-def _embed_bwd(L, tok_t=0, n=8, g_t=0, ld_g=16, vocab=256, d=16, t_t=0, ld_t=16, p=(A, A, A, A), ws=None):
+def _embed_bwd(L, tok_t=0, n=9000, g_t=0, ld_g=16, vocab=256, d=16, t_t=0, ld_t=16, p=(A, A, A, A), ws=None):
     ws = L.boa_embed_backward_workspace(n, vocab, d) if ws is None else ws
     return L.boa_embed_backward(p[0], tok_t, n, p[1], g_t, ld_g, vocab, d, 1.0, 0, p[2], t_t, ld_t, p[3], ws, None)
 
