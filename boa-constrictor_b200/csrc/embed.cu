@@ -55,10 +55,11 @@ embed_kernel(const Tok* __restrict__ tok, long long n, const TI* __restrict__ ta
       const int l = l0 + u * kEmbedThreads;
       if (l >= items) break;
       const int c = (l - row[u] * q) * N;
-      Pack<TO, N> o;
+      float o[N];
+      if (idx[u] >= 0) widen_pack(e[u], o);
 #pragma unroll
-      for (int k = 0; k < N; ++k) o.v[k] = from_f32<TO>(idx[u] >= 0 ? scale * to_f32(e[u].v[k]) : 0.f);
-      *reinterpret_cast<Pack<TO, N>*>(out + (r0 + row[u]) * ld_out + c) = o;
+      for (int k = 0; k < N; ++k) o[k] = idx[u] >= 0 ? scale * o[k] : 0.f;
+      *reinterpret_cast<Pack<TO, N>*>(out + (r0 + row[u]) * ld_out + c) = narrow_pack<TO>(o);
     }
   }
 }
@@ -157,9 +158,9 @@ cudaError_t launch_embed(const void* tokens, int tok_t, long long n, const void*
 
 // ---------------------------------------------------------------- gradient
 // Workspace, as 32-bit words: counts [V][tiles], then exclusive along the
-// tiles; total [V]; base [V + 1] and piece_base [V + 1], the first sorted
-// position and the first piece of each token; done [V], its finished pieces;
-// order [n]; and the pieces' sums [pieces][d] in fp32.
+// tiles; total [V]; done [V], finished pieces of each token; order [n];
+// pieces [most] of four words (and their number before them); and the pieces'
+// sums [most][d] in fp32.
 constexpr int kSortThreads = 256;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortHeld = 8;                               // tokens that a lane holds at once
@@ -173,8 +174,8 @@ constexpr int kSmallRows = 4096;   // up to here one kernel does all
 struct GradPlan {
   int tiles, tile;                 // tiles of the sort, tokens of a tile
   int rows;                        // rows of a piece (more for a token of over kMaxPieces * rows)
-  long long pieces;                // most pieces there can be
-  size_t counts, total, base, piece_base, done, order, part, words;  // offsets in words
+  long long most;                  // pieces there can be
+  size_t counts, total, done, order, pieces, part, words;  // offsets in words
 };
 static GradPlan grad_plan(long long n, int vocab, int d) {
   GradPlan p{};
@@ -182,32 +183,36 @@ static GradPlan grad_plan(long long n, int vocab, int d) {
   tile = (tile + kTile - 1) / kTile * kTile;
   p.tile = (int)tile;
   p.tiles = (int)((n + tile - 1) / tile);
-  // about eight blocks per SM
-  const long long rows = (n + 148 * 8 - 1) / (148 * 8);
+  // about sixteen blocks per SM
+  const long long rows = (n + 148 * 16 - 1) / (148 * 16);
   p.rows = (int)(rows < 128 ? 128 : (rows + 31) / 32 * 32);
-  p.pieces = n / p.rows + vocab;   // at least the sum of ceil(total / rows)
+  p.most = n / p.rows + vocab;     // at least the sum of pieces_of(total)
   auto up4 = [](size_t x) { return (x + 3) & ~(size_t)3; };
   p.counts = 0;
   p.total = up4(p.counts + (size_t)vocab * p.tiles);
-  p.base = up4(p.total + vocab);
-  p.piece_base = up4(p.base + vocab + 1);
-  p.done = up4(p.piece_base + vocab + 1);
+  p.done = up4(p.total + vocab);
   p.order = up4(p.done + vocab);
-  p.part = up4(p.order + (size_t)n);
-  p.words = p.part + (size_t)p.pieces * d;
+  p.pieces = up4(p.order + (size_t)n);
+  p.part = p.pieces + 4 * (size_t)(p.most + 1);
+  p.words = p.part + (size_t)p.most * d;
   return p;
 }
 size_t embed_grad_workspace(long long n, int vocab, int d) {
   return n > kSmallRows ? grad_plan(n, vocab, d).words * 4 : 0;
 }
-__host__ __device__ inline int rows_of_piece(int total, int rows) {
-  const int most = (total + kMaxPieces - 1) / kMaxPieces;
-  return most > rows ? most : rows;
+// Rows of a token's pieces, and their number (one, of no rows, for a token that does not occur).
+__device__ __forceinline__ int rows_of_piece(int total, int rows) {
+  return max(rows, (total + kMaxPieces - 1) / kMaxPieces);
 }
 __device__ __forceinline__ int pieces_of(int total, int rows) {
   const int r = rows_of_piece(total, rows);
-  return (total + r - 1) / r;
+  return max(1, (total + r - 1) / r);
 }
+struct alignas(16) Piece {
+  int tok_pieces;  // token, and its pieces << 16
+  int at, rows;    // sorted positions
+  int first;       // the token's first piece
+};
 
 // The tokens of 32 * kSortHeld positions from `at`, lane by lane; -1 past `end`.
 template <typename Tok>
@@ -320,17 +325,19 @@ __device__ __forceinline__ void vocab_prefix(const int* __restrict__ total, int 
   __syncthreads();
 }
 
-// Writes each position to its place in token order.  A warp takes its part of
+// Writes each position to its place in token order, and the pieces.  A warp takes its part of
 // the tile 32 tokens at a time: lanes that hold the same token find each
 // other with a match, so equal tokens keep the order of their positions.
 template <typename Tok>
 __global__ void __launch_bounds__(kSortThreads)
 embed_order_kernel(const Tok* __restrict__ tok, long long n, int vocab, int tile, int tiles, int rows,
-                   const int* __restrict__ counts, const int* __restrict__ total, int* __restrict__ base_out,
-                   int* __restrict__ piece_base, int* __restrict__ order) {
-  extern __shared__ int hist[];  // [kSortWarps][vocab] next places, base [vocab + 1], scratch [kSortWarps]
+                   const int* __restrict__ counts, const int* __restrict__ total, Piece* __restrict__ pieces,
+                   int* __restrict__ order) {
+  // [kSortWarps][vocab] next places, base and first piece [vocab + 1] each, scratch [kSortWarps]
+  extern __shared__ int hist[];
   int* base = hist + kSortWarps * vocab;
-  int* scratch = base + vocab + 1;
+  int* first = base + vocab + 1;
+  int* scratch = first + vocab + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int span = tile / kSortWarps;
   const long long w0 = (long long)blockIdx.x * tile + (long long)warp * span;
@@ -346,14 +353,15 @@ embed_order_kernel(const Tok* __restrict__ tok, long long n, int vocab, int tile
     for (int j = 0; j < kSortHeld; ++j)
       if (v[j] >= 0) atomicAdd(next + v[j], 1);
   }
-  if (blockIdx.x == 0) {  // the pieces of each token, for the kernel that follows
-    vocab_prefix(total, vocab, [&](int c) { return pieces_of(c, rows); }, base, scratch);
-    for (int k = threadIdx.x; k <= vocab; k += kSortThreads) piece_base[k] = base[k];
-    __syncthreads();
-  }
+  vocab_prefix(total, vocab, [&](int c) { return pieces_of(c, rows); }, first, scratch);
   vocab_prefix(total, vocab, [](int c) { return c; }, base, scratch);
-  if (blockIdx.x == 0)
-    for (int k = threadIdx.x; k <= vocab; k += kSortThreads) base_out[k] = base[k];
+  // the pieces, for the kernel that follows; pieces[0].at is their number
+  if (blockIdx.x == 0 && threadIdx.x == 0) pieces[0].at = first[vocab];
+  for (int k = blockIdx.x; k < vocab; k += gridDim.x) {
+    const int count = base[k + 1] - base[k], size = rows_of_piece(count, rows), n_pieces = first[k + 1] - first[k];
+    for (int j = threadIdx.x; j < n_pieces; j += kSortThreads)
+      pieces[1 + first[k] + j] = {k | n_pieces << 16, base[k] + j * size, max(0, min(size, count - j * size)), first[k]};
+  }
   for (int k = threadIdx.x; k < vocab; k += kSortThreads) {
     int at = base[k] + counts[(size_t)k * tiles + blockIdx.x];
 #pragma unroll
@@ -381,16 +389,6 @@ embed_order_kernel(const Tok* __restrict__ tok, long long n, int vocab, int tile
   }
 }
 
-// A pack of a row that is read once.
-template <typename T_, int N>
-__device__ __forceinline__ Pack<T_, N> load_once(const T_* p) {
-  if constexpr (N * sizeof(T_) == 16) {
-    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
-    return *reinterpret_cast<const Pack<T_, N>*>(&w);
-  } else {
-    return *reinterpret_cast<const Pack<T_, N>*>(p);
-  }
-}
 // out (+)= scale * sum of N columns
 template <typename TD, int N>
 __device__ __forceinline__ void store_grad(TD* out, const float (&sum)[N], float scale, int accumulate) {
@@ -416,43 +414,19 @@ __device__ __forceinline__ void join_groups(float (&acc)[N], float* s_sum, int g
 
 // Sum of one piece: the block's threads form groups of `per_row` threads, one
 // pack of N columns each; group g takes the piece's rows g, g + groups, ...
-// The block that finishes a token's pieces last adds them up; blocks beyond
-// the last piece see to the tokens that do not occur.
+// The block that finishes a token's pieces last adds them up.
 template <typename TG, typename TD, int N>
 __global__ void __launch_bounds__(kSumThreads)
-embed_sum_kernel(const TG* __restrict__ dout, long long ld, int vocab, int d, int per_row, int rows_least,
-                 const int* __restrict__ total, const int* __restrict__ base, const int* __restrict__ piece_base,
+embed_sum_kernel(const TG* __restrict__ dout, long long ld, int d, int per_row, const Piece* __restrict__ all,
                  const int* __restrict__ order, int* __restrict__ done, float* __restrict__ part, float scale,
                  int accumulate, TD* dtable, long long ld_dtable) {
-  __shared__ int s_tok, s_last, s_order[kSumChunk], scratch[kSumThreads / 32];
+  __shared__ int s_last, s_order[kSumChunk];
   __shared__ float s_sum[kSumThreads * N];
-  const int p = blockIdx.x, pieces_all = piece_base[vocab];
-  if (threadIdx.x == 0) s_tok = -1;
-  __syncthreads();
-  if (p >= pieces_all) {  // the (p - pieces_all)-th token that does not occur
-    if (accumulate) return;
-    constexpr int PER = kMaxVocab / kSumThreads;
-    int none = 0, all;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) none += threadIdx.x * PER + k < vocab && total[threadIdx.x * PER + k] == 0;
-    int at = block_prefix<kSumThreads>(none, scratch, all);
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int v = threadIdx.x * PER + k;
-      if (v < vocab && total[v] == 0 && at++ == p - pieces_all) s_tok = v;
-    }
-    __syncthreads();
-    if (s_tok >= 0)
-      for (int c = threadIdx.x; c < d; c += kSumThreads) dtable[s_tok * ld_dtable + c] = from_f32<TD>(0.f);
-    return;
-  }
-  for (int v = threadIdx.x; v < vocab; v += kSumThreads)
-    if (piece_base[v] <= p && p < piece_base[v + 1]) s_tok = v;
-  __syncthreads();
-  const int v = s_tok, count = total[v], first_piece = piece_base[v], pieces = piece_base[v + 1] - first_piece;
-  const int size = rows_of_piece(count, rows_least);
-  const int begin = (p - first_piece) * size, rows = min(size, count - begin);
-  const int* mine = order + base[v] + begin;
+  const int p = blockIdx.x;
+  const Piece me = all[1 + p];
+  if (p >= all[0].at) return;
+  const int v = me.tok_pieces & 0xffff, pieces = me.tok_pieces >> 16, rows = me.rows;
+  const int* mine = order + me.at;
   const int groups = kSumThreads / per_row, g = threadIdx.x / per_row, col = threadIdx.x - g * per_row;
   const int q = d / N;
   for (int c0 = 0; c0 < q; c0 += per_row) {
@@ -474,9 +448,10 @@ embed_sum_kernel(const TG* __restrict__ dout, long long ld, int vocab, int d, in
         const TG* x = dout + (size_t)c * N;
 #pragma unroll 8
         for (int r = g; r < here; r += groups) {
-          const Pack<TG, N> y = load_once<TG, N>(x + s_order[r] * ld);
+          float y[N];
+          widen_pack(load_once<TG, N>(x + s_order[r] * ld), y);
 #pragma unroll
-          for (int k = 0; k < N; ++k) acc[k] += to_f32(y.v[k]);
+          for (int k = 0; k < N; ++k) acc[k] += y[k];
         }
       }
     }
@@ -503,7 +478,7 @@ embed_sum_kernel(const TG* __restrict__ dout, long long ld, int vocab, int d, in
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
     if (g < groups && c < q) {
-      const float* x = part + (size_t)first_piece * d + c * N;
+      const float* x = part + (size_t)me.first * d + c * N;
 #pragma unroll 8
       for (int r = g; r < pieces; r += groups)
 #pragma unroll
@@ -566,9 +541,10 @@ embed_small_kernel(const Tok* __restrict__ tok, int n, const TG* __restrict__ do
       const TG* x = dout + (size_t)(c0 + col) * N;
 #pragma unroll 8
       for (int r = g; r < rows; r += groups) {
-        const Pack<TG, N> y = load_once<TG, N>(x + s_order[r] * ld);
+        float y[N];
+        widen_pack(load_once<TG, N>(x + s_order[r] * ld), y);
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += to_f32(y.v[k]);
+        for (int k = 0; k < N; ++k) acc[k] += y[k];
       }
     }
     join_groups<N>(acc, s_sum, g, groups, col, packs);
@@ -598,11 +574,12 @@ static cudaError_t grad_run(const Tok* tok, long long n, const TG* dout, long lo
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   embed_prefix_kernel<<<vocab, kPrefixThreads, 0, st>>>(w + p.counts, p.tiles, w + p.total, w + p.done);
-  embed_order_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes + (vocab + 1 + kSortWarps) * 4, st>>>(
-      tok, n, vocab, p.tile, p.tiles, p.rows, w + p.counts, w + p.total, w + p.base, w + p.piece_base, w + p.order);
-  embed_sum_kernel<TG, TD, N><<<(unsigned)p.pieces, kSumThreads, 0, st>>>(
-      dout, ld, vocab, d, q < kSumThreads ? q : kSumThreads, p.rows, w + p.total, w + p.base, w + p.piece_base,
-      w + p.order, w + p.done, reinterpret_cast<float*>(w + p.part), scale, accumulate ? 1 : 0, dtable, ld_dtable);
+  Piece* pieces = reinterpret_cast<Piece*>(w + p.pieces);
+  embed_order_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes + (2 * (vocab + 1) + kSortWarps) * 4, st>>>(
+      tok, n, vocab, p.tile, p.tiles, p.rows, w + p.counts, w + p.total, pieces, w + p.order);
+  embed_sum_kernel<TG, TD, N><<<(unsigned)p.most, kSumThreads, 0, st>>>(
+      dout, ld, d, q < kSumThreads ? q : kSumThreads, pieces, w + p.order, w + p.done,
+      reinterpret_cast<float*>(w + p.part), scale, accumulate ? 1 : 0, dtable, ld_dtable);
   return cudaGetLastError();
 }
 

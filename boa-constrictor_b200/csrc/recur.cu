@@ -63,17 +63,6 @@ __device__ __forceinline__ uint32_t div_by(uint32_t n, FastDiv f) {
   return f.d == 1 ? n : __umulhi(n, f.mul) >> f.shift;
 }
 
-__device__ __forceinline__ float ex2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp_fast(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // V chains of a lane.  (Packed pairs, f32x2, were measured slower: they run on
 // one of the two FMA pipes only, and most of the arithmetic here is FMA work.)
 template <int V>
@@ -126,7 +115,6 @@ struct Cell {
 };
 template <int V, bool GRAD>
 __device__ __forceinline__ Cell<V> mingru_cell(const Vec<V>& zl, const Vec<V>& hr) {
-  constexpr float kLog2e = 1.44269504f;
   Cell<V> k;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -335,27 +323,10 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Packs as fp32 and back.  Pairs of 16 bits are taken as the 32-bit word that
-// they are: taken as two halves they cost twice the instructions.
 template <typename T_, int V>
 __device__ __forceinline__ Vec<V> widen(const Pack<T_, V>& p) {
   Vec<V> r;
-  if constexpr (V == 2 && sizeof(T_) == 2) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(&p);
-    if constexpr (std::is_same<T_, __nv_bfloat16>::value) {
-      r.v[0] = __uint_as_float(w << 16);
-      r.v[1] = __uint_as_float(w & 0xffff0000u);
-    } else {
-      __half2 h;
-      *reinterpret_cast<uint32_t*>(&h) = w;
-      const float2 f = __half22float2(h);
-      r.v[0] = f.x;
-      r.v[1] = f.y;
-    }
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) r.v[v] = to_f32(p.v[v]);
-  }
+  widen_pack(p, r.v);
   return r;
 }
 // a row that is not there as `fill`
@@ -368,22 +339,7 @@ __device__ __forceinline__ Vec<V> widen(const Pack<T_, V>& p, bool there, float 
 }
 template <typename T_, int V>
 __device__ __forceinline__ void store_rounded(T_* to, const Vec<V>& x) {
-  if constexpr (V == 2 && sizeof(T_) == 2) {
-    uint32_t w;
-    if constexpr (std::is_same<T_, __nv_bfloat16>::value) {
-      const __nv_bfloat162 r = __floats2bfloat162_rn(x.v[0], x.v[1]);
-      w = *reinterpret_cast<const uint32_t*>(&r);
-    } else {
-      const __half2 r = __floats2half2_rn(x.v[0], x.v[1]);
-      w = *reinterpret_cast<const uint32_t*>(&r);
-    }
-    *reinterpret_cast<uint32_t*>(to) = w;
-  } else {
-    Pack<T_, V> p;
-#pragma unroll
-    for (int v = 0; v < V; ++v) p.v[v] = from_f32<T_>(x.v[v]);
-    *reinterpret_cast<Pack<T_, V>*>(to) = p;
-  }
+  *reinterpret_cast<Pack<T_, V>*>(to) = narrow_pack<T_>(x.v);
 }
 
 // A lane's packs of a stage: [stream][P][32] of its warp, so that the offsets

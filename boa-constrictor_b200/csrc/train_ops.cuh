@@ -40,6 +40,79 @@ struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
   T v[N];
 };
 
+// A pack as fp32 and back.  Pairs of 16 bits are taken as the 32-bit words that
+// they are: taken as halves they cost twice the instructions.
+template <typename T, int N>
+__device__ __forceinline__ void widen_pack(const Pack<T, N>& p, float (&r)[N]) {
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        r[2 * k] = __uint_as_float(w[k] << 16);
+        r[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+      } else {
+        __half2 h;
+        *reinterpret_cast<uint32_t*>(&h) = w[k];
+        const float2 f = __half22float2(h);
+        r[2 * k] = f.x;
+        r[2 * k + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) r[k] = to_f32(p.v[k]);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> narrow_pack(const float (&x)[N]) {
+  Pack<T, N> p;
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&r);
+      } else {
+        const __half2 r = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+        w[k] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) p.v[k] = from_f32<T>(x[k]);
+  }
+  return p;
+}
+// A pack that is read once, or written and not read again here.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_once(const T* p) {
+  if constexpr (N * sizeof(T) == 16) {
+    const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
+    return *reinterpret_cast<const Pack<T, N>*>(&w);
+  } else {
+    return *reinterpret_cast<const Pack<T, N>*>(p);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_once(T* p, const Pack<T, N>& x) {
+  if constexpr (N * sizeof(T) == 16) __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&x));
+  else *reinterpret_cast<Pack<T, N>*>(p) = x;
+}
+// 2^x and 1 / x to about one step of fp32; results below 2^-126 are 0
+__device__ __forceinline__ float ex2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.44269504f;
+
 // A token as an index, or -1 when it lies outside [0, vocab): such a token
 // pads a batch, and no address is formed from it.
 template <typename Tok>
