@@ -304,13 +304,17 @@ __device__ __forceinline__ void leave(const Walk<V>& K, const Place& p, int pari
   if (p.ranks == 1 && (REVERSE ? p.warp == 0 : p.warp == p.warps - 1)) K.state[(parity ^ 1) * 32 + p.lane] = s;
 }
 
-// Rows on their way from HBM: every lane copies the packs that it will use
-// itself into its own places of shared memory, so only its own copies need to
-// be waited for.  A pack of 2 bytes (odd widths) is too small for an
-// asynchronous copy and is moved by a load and a store.
+// Rows on their way from HBM to a warp's stage, [row][32 lanes] packs a
+// stream.  QUADS: 16 bytes a lane, several rows an instruction, where every
+// row lets them be moved whole (a lane then brings packs that other lanes of
+// its warp use).  Otherwise every lane brings its own packs; one of 2 bytes
+// (odd widths) is too small for an asynchronous copy and is moved by a load
+// and a store.
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
-  if constexpr (BYTES >= 4) {
+  if constexpr (BYTES == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  } else if constexpr (BYTES >= 4) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
   } else {
     const unsigned short x = __ldg(static_cast<const unsigned short*>(from));
@@ -342,11 +346,10 @@ __device__ __forceinline__ void store_rounded(T_* to, const Vec<V>& x) {
   *reinterpret_cast<Pack<T_, V>*>(to) = narrow_pack<T_>(x.v);
 }
 
-// A lane's packs of a stage: [stream][P][32] of its warp, so that the offsets
-// of the rows are constants.
+// A warp's stages, [stage][stream][P][32].
 template <typename T_, int V, int P, int STREAMS>
 __device__ __forceinline__ Pack<T_, V>* warp_stages(uint8_t* stages, int S) {
-  return reinterpret_cast<Pack<T_, V>*>(stages) + (threadIdx.x >> 5) * (S * STREAMS * P * 32) + (threadIdx.x & 31);
+  return reinterpret_cast<Pack<T_, V>*>(stages) + (threadIdx.x >> 5) * (S * STREAMS * P * 32);
 }
 // row p after `x`, `row` bytes each: one multiply-add of 32 bits to 64
 template <typename P_>
@@ -354,19 +357,41 @@ __device__ __forceinline__ P_* row_at(P_* x, uint32_t row, int p) {
   using B_ = typename std::conditional<std::is_const<P_>::value, const char, char>::type;
   return reinterpret_cast<P_*>(reinterpret_cast<B_*>(x) + (unsigned long long)row * (uint32_t)p);
 }
-template <int P, typename T_, int V>
-__device__ __forceinline__ void copy_rows(Pack<T_, V>* to, const T_* x, uint32_t row, int live, bool whole) {
-  const uint32_t at = smem_u32(to);
-  if (whole) {
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      copy_async<sizeof(T_) * V>(at + p * 32 * (int)sizeof(Pack<T_, V>), row_at(x, row, p));
-  } else {
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (p < live) copy_async<sizeof(T_) * V>(at + p * 32 * (int)sizeof(Pack<T_, V>), row_at(x, row, p));
+// Which part of a warp's rows a lane brings: elements `c` on of chunk `b`, of
+// rows first, first + EVERY, ...; `at` bytes into the stage.
+template <typename T_, int V, bool QUADS>
+struct Carrier {
+  static constexpr int kBytes = QUADS ? 16 : (int)sizeof(T_) * V;
+  static constexpr int kRow = 32 * (int)sizeof(T_) * V;      // bytes of a row in the stage
+  static constexpr int kEvery = 32 * kBytes / kRow;          // rows of an instruction
+  int b, c, first, len;
+  uint32_t at;
+  __device__ __forceinline__ Carrier(const Place& p, int T, int d, FastDiv by_d, long long chains, const int* lengths) {
+    const int piece = p.lane % (32 / kEvery);
+    first = p.lane / (32 / kEvery);
+    at = (uint32_t)(p.lane * kBytes);
+    const long long chain = p.chain - p.lane * V + piece * (kBytes / (int)sizeof(T_));
+    const bool in = chain < chains;
+    b = in ? (int)div_by((uint32_t)chain, by_d) : 0;
+    c = in ? (int)(chain - (long long)b * d) : 0;
+    len = in ? T : 0;
+    if (in && lengths) len = min(max(lengths[b], 0), T);
   }
-}
+  // the rows of [t, t + P) that are there (`whole`: all); x is at row t + first
+  template <int P>
+  __device__ __forceinline__ void copy(Pack<T_, V>* stage, const T_* x, uint32_t row, int t, bool whole) const {
+    const uint32_t to = smem_u32(stage) + at;
+    if (whole) {
+#pragma unroll
+      for (int k = 0; k < P / kEvery; ++k) copy_async<kBytes>(to + k * kEvery * kRow, row_at(x, row, k * kEvery));
+    } else {
+#pragma unroll
+      for (int k = 0; k < P / kEvery; ++k)
+        if (t + first + k * kEvery < len)
+          copy_async<kBytes>(to + k * kEvery * kRow, row_at(x, row, k * kEvery));
+    }
+  }
+};
 // rows of [from, from + P) before `end`
 template <int P>
 __device__ __forceinline__ int rows_left(int from, int end) { return max(min(P, end - from), 0); }
@@ -378,7 +403,7 @@ constexpr int kStages = 2;  // the step in use, and the next one on its way
 // A warp whose rows are all there (`whole`, the same for its lanes) takes a
 // form without those tests.
 // ------------------------------------------------------------------ forward
-template <typename T_, int V>
+template <typename T_, int V, bool QUADS>
 __global__ void __maxnreg__((scan_regs<T_, V>()))
 mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains,
                    const int* __restrict__ lengths, const float* h0, T_* __restrict__ h, RowStrides hs,
@@ -394,7 +419,8 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
   const int all_len = __reduce_min_sync(~0u, len);  // positions that all of the warp's chains have
   const int step = ranks * warps * P;  // positions of a step of the walk
   int t = (at.rank * warps + at.warp) * P;
-  const T_* x = zh + at.b * zs.chunk + t * zs.row + at.c;
+  const Carrier<T_, V, QUADS> by(at, T, d, by_d, chains, lengths);
+  const T_* x = zh + by.b * zs.chunk + (t + by.first) * zs.row + by.c;
   T_* o = h + at.b * hs.chunk + t * hs.row + at.c;
   Pack<T_, V>* const stages = warp_stages<T_, V, P, 2>(K.stages, S);
   const long long x_step = step * zs.row, o_step = step * hs.row;
@@ -403,10 +429,9 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
   int t_next = t, put = 0, got = 0;  // the next step to fetch, its stage, and the stage in use
   auto fetch = [&](bool more) {
     if (more) {
-      const int live = rows_left<P>(t_next, len);
       const bool whole = t_next + P <= all_len;
-      copy_rows<P>(stages + put * STAGE, x, x_row, live, whole);
-      copy_rows<P>(stages + put * STAGE + P * 32, x + d, x_row, live, whole);
+      by.template copy<P>(stages + put * STAGE, x, x_row, t_next, whole);
+      by.template copy<P>(stages + put * STAGE + P * 32, x + d, x_row, t_next, whole);
       x += x_step;
       t_next += step;
       put = put + 1 == S ? 0 : put + 1;
@@ -422,7 +447,8 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     for (int v = 0; v < V; ++v) walk.v[v] = h0[at.chain + v];
   for (int i = 0; i < steps; ++i) {
     copies_wait<S - 2>();
-    const Pack<T_, V>*zl = stages + got * STAGE, *hr = zl + P * 32;
+    __syncwarp();  // the other lanes' copies too
+    const Pack<T_, V>*zl = stages + got * STAGE + at.lane, *hr = zl + P * 32;
     got = got + 1 == S ? 0 : got + 1;
     const int live = rows_left<P>(t, len), rows = rows_left<P>(t, end);
     const bool whole = t + P <= all_len;
@@ -470,7 +496,7 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
 }
 
 // ----------------------------------------------------------------- backward
-template <typename T_, int V>
+template <typename T_, int V, bool QUADS>
 __global__ void __maxnreg__(kGradRegs)
 mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains,
                    const int* __restrict__ lengths, const float* __restrict__ states, const T_* __restrict__ dh,
@@ -491,8 +517,9 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
   int t = (steps - 1) * step + (at.rank * warps + at.warp) * P;
   // the warps between the saved state and this warp's positions
   const int lead = at.warp % min(warps, kSpan / P);
-  const T_* x = zh + at.b * zs.chunk + t * zs.row + at.c;
-  const T_* u = dh + at.b * dhs.chunk + t * dhs.row + at.c;
+  const Carrier<T_, V, QUADS> by(at, T, d, by_d, chains, lengths);
+  const T_* x = zh + by.b * zs.chunk + (t + by.first) * zs.row + by.c;
+  const T_* u = dh + by.b * dhs.chunk + (t + by.first) * dhs.row + by.c;
   T_* o = dzh + at.b * dzs.chunk + t * dzs.row + at.c;
   const long long x_step = step * zs.row, u_step = step * dhs.row, o_step = step * dzs.row;
   const uint32_t x_row = (uint32_t)(zs.row * sizeof(T_)), u_row = (uint32_t)(dhs.row * sizeof(T_)),
@@ -502,11 +529,10 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
   int t_next = t, put = 0, got = 0;  // the next step to fetch, its stage, and the stage in use
   auto fetch = [&](bool more) {
     if (more) {
-      const int live = rows_left<P>(t_next, len);
       const bool whole = t_next + P <= all_len;
-      copy_rows<P>(stages + put * STAGE, x, x_row, live, whole);
-      copy_rows<P>(stages + put * STAGE + P * 32, x + d, x_row, live, whole);
-      copy_rows<P>(stages + put * STAGE + 2 * P * 32, u, u_row, live, whole);
+      by.template copy<P>(stages + put * STAGE, x, x_row, t_next, whole);
+      by.template copy<P>(stages + put * STAGE + P * 32, x + d, x_row, t_next, whole);
+      by.template copy<P>(stages + put * STAGE + 2 * P * 32, u, u_row, t_next, whole);
       x -= x_step;
       u -= u_step;
       t_next -= step;
@@ -529,7 +555,8 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     for (int v = 0; v < V; ++v) walk.v[v] = dh_last[at.chain + v];
   for (int i = 0; i < steps; ++i) {
     copies_wait<S - 2>();
-    const Pack<T_, V>*zl = stages + got * STAGE, *hr = zl + P * 32, *du = hr + P * 32;
+    __syncwarp();  // the other lanes' copies too, and all have read the stage that is filled next
+    const Pack<T_, V>*zl = stages + got * STAGE + at.lane, *hr = zl + P * 32, *du = hr + P * 32;
     got = got + 1 == S ? 0 : got + 1;
     const int live = rows_left<P>(t, len), rows = rows_left<P>(t, end);
     Vec<V> s = next_saved;
@@ -644,11 +671,12 @@ mingru_step_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
 }
 
 // ------------------------------------------------------------------ launches
-// Two chains per lane where every row lets pairs be moved whole.
-static bool pairs_ok(int d, int type, std::initializer_list<std::pair<const void*, RowStrides>> rows) {
-  if (d % 2) return false;
+// Whether every row lets `n` elements be moved whole: the pointers and strides
+// are multiples of them, and so is d.
+static bool moved_whole(int n, int d, int type, std::initializer_list<std::pair<const void*, RowStrides>> rows) {
+  if (d % n) return false;
   for (const auto& r : rows)
-    if (r.second.row % 2 || r.second.chunk % 2 || !aligned_to(r.first, 2 * type_bytes(type))) return false;
+    if (r.second.row % n || r.second.chunk % n || !aligned_to(r.first, n * type_bytes(type))) return false;
   return true;
 }
 
@@ -724,13 +752,15 @@ cudaError_t launch_mingru_scan(const void* zh, int type, RowStrides zs, int B, i
                                cudaStream_t st) {
   const long long chains = (long long)B * d;
   const FastDiv by_d = fast_div((uint32_t)d);
-  const bool pairs = pairs_ok(d, type, {{zh, zs}, {h, hs}});
+  const bool pairs = moved_whole(2, d, type, {{zh, zs}, {h, hs}});
+  const bool quads = moved_whole(16 / type_bytes(type), d, type, {{zh, zs}});
   return with_type(type, [&](auto t) {
     using E = decltype(t);
     const E* x = static_cast<const E*>(zh);
     E* o = static_cast<E*>(h);
-    auto go = [&](auto vec) -> cudaError_t {
+    auto go = [&](auto vec, auto whole) -> cudaError_t {
       constexpr int V = decltype(vec)::value;
+      constexpr bool Q = decltype(whole)::value;
       if (T <= kFew) {
         const unsigned blocks = (unsigned)((chains + 256 * V - 1) / (256 * V));
         if (T <= 1)
@@ -744,11 +774,16 @@ cudaError_t launch_mingru_scan(const void* zh, int type, RowStrides zs, int B, i
       auto smem = [](int w, int ranks) {
         return Walk<V>::bytes(w, ranks, false) + (size_t)kStages * 2 * scan_steps<E, V>() * w * 32 * sizeof(Pack<E, V>);
       };
-      return launch_walk<V>(mingru_scan_kernel<E, V>, chains, T, scan_steps<E, V>(), smem, st, x, zs, T, d, by_d, chains,
+      return launch_walk<V>(mingru_scan_kernel<E, V, Q>, chains, T, scan_steps<E, V>(), smem, st, x, zs, T, d, by_d, chains,
                             lengths, h0, o, hs, h_last, states);
     };
-    return pairs && (sizeof(E) == 2 || T <= kFew || chains >= 148 * 64) ? go(std::integral_constant<int, 2>{})
-                                                        : go(std::integral_constant<int, 1>{});
+    // two chains a lane: always for 16 bits; for 32 bits where that leaves
+    // groups enough to fill the GPU
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    if (pairs && (sizeof(E) == 2 || T <= kFew || chains >= 148 * 64))
+      return quads && T > kFew ? go(two, std::true_type{}) : go(two, std::false_type{});
+    return sizeof(E) == 4 && quads ? go(one, std::true_type{}) : go(one, std::false_type{});
   });
 }
 
@@ -762,19 +797,24 @@ cudaError_t launch_mingru_scan_grad(const void* zh, int type, RowStrides zs, int
                    : cudaMemsetAsync(dh0, 0, (size_t)chains * 4, st);
   }
   const FastDiv by_d = fast_div((uint32_t)d);
-  const bool pairs = pairs_ok(d, type, {{zh, zs}, {dh, dhs}, {dzh, dzs}});
+  const bool pairs = moved_whole(2, d, type, {{zh, zs}, {dh, dhs}, {dzh, dzs}});
+  const bool quads = moved_whole(16 / type_bytes(type), d, type, {{zh, zs}, {dh, dhs}});
   return with_type(type, [&](auto t) {
     using E = decltype(t);
-    auto go = [&](auto vec) {
+    auto go = [&](auto vec, auto whole) {
       constexpr int V = decltype(vec)::value;
+      constexpr bool Q = decltype(whole)::value;
       auto smem = [](int w, int ranks) {
         return Walk<V>::bytes(w, ranks, true) + (size_t)kStages * 3 * kGradSteps * w * 32 * sizeof(Pack<E, V>);
       };
-      return launch_walk<V>(mingru_grad_kernel<E, V>, chains, T, kGradSteps, smem, st, static_cast<const E*>(zh), zs,
+      return launch_walk<V>(mingru_grad_kernel<E, V, Q>, chains, T, kGradSteps, smem, st, static_cast<const E*>(zh), zs,
                             T, d, by_d, chains, lengths, states, static_cast<const E*>(dh), dhs, dh_last,
                             static_cast<E*>(dzh), dzs, dh0);
     };
-    return pairs && sizeof(E) == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    if (pairs && sizeof(E) == 2) return quads ? go(two, std::true_type{}) : go(two, std::false_type{});
+    return sizeof(E) == 4 && quads ? go(one, std::true_type{}) : go(one, std::false_type{});
   });
 }
 
