@@ -37,16 +37,18 @@ constexpr int kMaxWarps = 16;    // warps of a block
 constexpr int kMaxCluster = 8;    // blocks of a cluster (the portable limit)
 constexpr int kFew = 8;           // up to here, one thread takes a chain through all positions
 // Positions that a warp holds, and registers a thread, for V chains a lane.
-// Longer runs spread the exchange over more positions; fewer registers let
-// more warps hide each other's latencies.  Four-byte pairs have the bytes to
-// wait for, so there the warps win (256 x 1024 x 256 forward: 4 positions at 56
-// registers 143 us, 8 at 80 169 us); two-byte pairs are paced by instructions
-// (64 x 4096 x 256 forward: 165 us and 129 us).
+// Long runs spread the exchange and the walk's bookkeeping over more
+// positions, which is what paces 16-bit rows and few chains (32 x 4096 x 256
+// bf16 forward: 8 positions at 80 registers 69 us, 16 at 128 60 us).  With many
+// 32-bit chains there are bytes enough to wait for, and more warps win
+// (256 x 1024 x 256 forward: 4 positions at 56 registers 143 us, 8 at 80
+// 169 us).  Backward a position holds twice the values (8 at 128: 95 us, 4 at
+// 80: 134 us).
 template <typename T_, int V>
-constexpr int scan_steps() { return V == 2 && sizeof(T_) == 4 ? 4 : 8; }
+constexpr int scan_steps() { return V == 2 && sizeof(T_) == 4 ? 4 : 16; }
 template <typename T_, int V>
-constexpr int scan_regs() { return V == 2 && sizeof(T_) == 4 ? 56 : 80; }
-constexpr int kGradSteps = 8, kGradRegs = 112;
+constexpr int scan_regs() { return V == 1 ? 96 : sizeof(T_) == 4 ? 56 : 128; }
+constexpr int kGradSteps = 8, kGradRegs = 128;
 
 // n / d for n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and
 // mul = floor(2^(31+s) / d) + 1, mul d exceeds 2^(31+s) by at most d, and
