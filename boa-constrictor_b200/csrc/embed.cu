@@ -3,9 +3,7 @@
 //   out[i] = s * E[t_i]          dE[v] = s * sum_{i : t_i = v} dout[i]
 //
 // Lookup.  n * d elements leave, and the table (at most 1024 rows) is read
-// from the caches, so the stores set the pace.  Where there are many more rows
-// than the table has, a block keeps a slice of the table's columns in shared
-// memory, scaled and rounded, and every row leaves by one bulk copy.
+// from the caches, so the stores set the pace.
 //
 // Gradient.  Every row of dout is read once, whatever its token: the
 // positions are first ordered by token with a stable counting sort (at most
@@ -23,111 +21,66 @@
 namespace boa {
 
 // ------------------------------------------------------------------ lookup
-// A block writes `rows` rows of q packs of N elements; thread k takes packs
-// k, k + 256, ...  The row of pack l is umulhi(l, magic) with
-// magic = ceil(2^32 / q), exact while l * q < 2^32.
+// A block writes `rows` rows; an item of a row is H packs of N elements, d / H
+// apart, and thread k takes items k, k + 256, ... of the block's rows * q.  The
+// row of item l is umulhi(l, magic) with magic = ceil(2^32 / q), exact while
+// l * q < 2^32.  A pack has 16 bytes in the wider of the two types: with more, a
+// warp's loads from the table would skip every other 16 bytes and take twice
+// the L1 cycles.
 constexpr int kEmbedThreads = 256;
-constexpr int kEmbedUnroll = 4;
 
-template <typename Tok, typename TI, typename TO, int N>
+template <typename Tok, typename TI, typename TO, int N, int H, int U>
 __global__ void __launch_bounds__(kEmbedThreads)
 embed_kernel(const Tok* __restrict__ tok, long long n, const TI* __restrict__ table, long long ld_table, int vocab,
              int q, uint32_t magic, int rows, float scale, TO* __restrict__ out, long long ld_out) {
   const long long r0 = (long long)blockIdx.x * rows;
   const int here = (int)(n - r0 < rows ? n - r0 : rows);
-  const int items = here * q;
-  for (int l0 = threadIdx.x; l0 < items; l0 += kEmbedThreads * kEmbedUnroll) {
-    int row[kEmbedUnroll], idx[kEmbedUnroll];
-    Pack<TI, N> e[kEmbedUnroll];
+  const int items = here * q, apart = q * N;
+  for (int l0 = threadIdx.x; l0 < items; l0 += kEmbedThreads * U) {
+    int row[U], idx[U];
+    Pack<TI, N> e[U][H];
 #pragma unroll
-    for (int u = 0; u < kEmbedUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int l = l0 + u * kEmbedThreads;
       row[u] = q == 1 ? l : (int)__umulhi((uint32_t)l, magic);
       idx[u] = l < items ? token_index(tok[r0 + row[u]], vocab) : -1;
     }
 #pragma unroll
-    for (int u = 0; u < kEmbedUnroll; ++u) {
-      const int c = (l0 + u * kEmbedThreads - row[u] * q) * N;
-      if (idx[u] >= 0) e[u] = *reinterpret_cast<const Pack<TI, N>*>(table + idx[u] * ld_table + c);
+    for (int u = 0; u < U; ++u) {
+      const TI* from = table + idx[u] * ld_table + (l0 + u * kEmbedThreads - row[u] * q) * N;
+#pragma unroll
+      for (int k = 0; k < H; ++k)
+        if (idx[u] >= 0) e[u][k] = *reinterpret_cast<const Pack<TI, N>*>(from + k * apart);
     }
 #pragma unroll
-    for (int u = 0; u < kEmbedUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int l = l0 + u * kEmbedThreads;
       if (l >= items) break;
-      const int c = (l - row[u] * q) * N;
-      float o[N];
-      if (idx[u] >= 0) widen_pack(e[u], o);
+      TO* to = out + (r0 + row[u]) * ld_out + (l - row[u] * q) * N;
 #pragma unroll
-      for (int k = 0; k < N; ++k) o[k] = idx[u] >= 0 ? scale * o[k] : 0.f;
-      *reinterpret_cast<Pack<TO, N>*>(out + (r0 + row[u]) * ld_out + c) = narrow_pack<TO>(o);
+      for (int k = 0; k < H; ++k) {
+        float o[N];
+        if (idx[u] >= 0) widen_pack(e[u][k], o);
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = idx[u] >= 0 ? scale * o[j] : 0.f;
+        *reinterpret_cast<Pack<TO, N>*>(to + k * apart) = narrow_pack<TO>(o);
+      }
     }
   }
 }
 
-template <typename Tok, typename TI, typename TO, int N>
+template <typename Tok, typename TI, typename TO, int N, int H, int U>
 static cudaError_t embed_run(const Tok* tok, long long n, const TI* table, long long ld_table, int vocab, int d,
                              float scale, TO* out, long long ld_out, cudaStream_t st) {
-  const int q = d / N;
-  // about two rounds of kEmbedThreads * kEmbedUnroll packs per block
-  int rows = 2 * kEmbedThreads * kEmbedUnroll / q;
+  const int q = d / (N * H);
+  // about two rounds of kEmbedThreads * U items per block
+  int rows = 2 * kEmbedThreads * U / q;
   rows = rows < 1 ? 1 : rows;
   const long long blocks = (n + rows - 1) / rows;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   const uint32_t magic = (uint32_t)(((1ull << 32) + q - 1) / q);
-  embed_kernel<Tok, TI, TO, N><<<(unsigned)blocks, kEmbedThreads, 0, st>>>(tok, n, table, ld_table, vocab, q, magic,
-                                                                           rows, scale, out, ld_out);
-  return cudaGetLastError();
-}
-
-// Many rows: block (slice, part) holds columns [c0, c0 + cols) of the table in
-// shared memory as they will be stored, with a row of zeros behind them for
-// padding, and sends one bulk copy per row.  The rows of a part go round the
-// warps 32 at a time.
-template <typename Tok, typename TI, typename TO>
-__global__ void __launch_bounds__(kEmbedThreads)
-embed_rows_kernel(const Tok* __restrict__ tok, long long n, const TI* __restrict__ table, long long ld_table,
-                  int vocab, int d, int cols, int slices, float scale, TO* __restrict__ out, long long ld_out) {
-  extern __shared__ __align__(128) uint8_t embed_smem[];
-  TO* rows = reinterpret_cast<TO*>(embed_smem);
-  const int slice = blockIdx.x % slices, part = blockIdx.x / slices, parts = gridDim.x / slices;
-  const int c0 = slice * cols, here = min(cols, d - c0);
-  for (int v = threadIdx.x >> 5; v <= vocab; v += kEmbedThreads / 32)
-    for (int c = threadIdx.x & 31; c < here; c += 32)
-      rows[v * cols + c] = from_f32<TO>(v < vocab ? scale * to_f32(table[v * ld_table + c0 + c]) : 0.f);
-  fence_proxy_async_smem();
-  __syncthreads();
-  const uint32_t bytes = (uint32_t)(here * sizeof(TO));
-  const long long stride = (long long)parts * kEmbedThreads;
-  for (long long i = (long long)part * kEmbedThreads + threadIdx.x; i < n; i += stride) {
-    const int v = token_index(tok[i], vocab);
-    bulk_store(out + i * ld_out + c0, rows + (v < 0 ? vocab : v) * cols, bytes);
-    bulk_commit();
-  }
-  bulk_wait_all();
-}
-constexpr int kEmbedSmem = 200 * 1024;
-// Columns of a slice: 16-byte multiples, so that vocab + 1 rows fit, and as
-// even as can be.  0 where a slice would be under 256 bytes.
-template <typename TO>
-static int embed_slice(int vocab, int d, int& slices) {
-  const int unit = 16 / (int)sizeof(TO), units = d / unit;
-  const int fit = kEmbedSmem / ((vocab + 1) * 16);
-  if (fit < 16 && fit < units) return 0;
-  slices = (units + fit - 1) / fit;
-  const int each = (units + slices - 1) / slices;
-  slices = (units + each - 1) / each;  // none is empty
-  return each * unit;
-}
-template <typename Tok, typename TI, typename TO>
-static cudaError_t embed_rows_run(const Tok* tok, long long n, const TI* table, long long ld_table, int vocab, int d,
-                                  int cols, int slices, float scale, TO* out, long long ld_out, cudaStream_t st) {
-  const size_t smem = (size_t)(vocab + 1) * cols * sizeof(TO);
-  const auto kernel = embed_rows_kernel<Tok, TI, TO>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  const int blocks = 148 * (int)(smem <= 110 * 1024 ? 2 : 1) / slices * slices;
-  kernel<<<(unsigned)(blocks < slices ? slices : blocks), kEmbedThreads, smem, st>>>(tok, n, table, ld_table, vocab, d,
-                                                                                    cols, slices, scale, out, ld_out);
+  embed_kernel<Tok, TI, TO, N, H, U><<<(unsigned)blocks, kEmbedThreads, 0, st>>>(
+      tok, n, table, ld_table, vocab, q, magic, rows, scale, out, ld_out);
   return cudaGetLastError();
 }
 
@@ -140,17 +93,23 @@ cudaError_t launch_embed(const void* tokens, int tok_t, long long n, const void*
         using Tok = decltype(tk);
         using TI = decltype(ti);
         using TO = decltype(to);
-        constexpr int N = 16 / sizeof(TO);
+        constexpr int N = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO));
         const Tok* t = static_cast<const Tok*>(tokens);
         const TI* e = static_cast<const TI*>(table);
         TO* o = static_cast<TO*>(out);
-        const bool wide = d % N == 0 && ld_out % N == 0 && ld_table % N == 0 && aligned_to(o, 16) &&
-                          aligned_to(e, (int)alignof(Pack<TI, N>));
-        if (!wide) return embed_run<Tok, TI, TO, 1>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
-        int slices = 1;
-        const int cols = n >= 1024ll * vocab ? embed_slice<TO>(vocab, d, slices) : 0;
-        return cols ? embed_rows_run<Tok, TI, TO>(t, n, e, ld_table, vocab, d, cols, slices, scale, o, ld_out, st)
-                    : embed_run<Tok, TI, TO, N>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
+        const bool wide = d % N == 0 && ld_out % N == 0 && ld_table % N == 0 &&
+                          aligned_to(o, (int)alignof(Pack<TO, N>)) && aligned_to(e, (int)alignof(Pack<TI, N>));
+        // Four packs an item share a token's lookup where rows are long (1M x 512,
+        // fp32 table, bf16 out: 177 us, two 198 us, one 276 us); short rows want
+        // items of more rows at once instead (1M x 64 bf16: two packs 31 us, four
+        // 40 us; 1M x 16 fp32: one 13.5 us, two 17 us).
+        const int packs = d / N;
+        if (!wide) return embed_run<Tok, TI, TO, 1, 1, 4>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
+        if (packs >= 64 && packs % 4 == 0)
+          return embed_run<Tok, TI, TO, N, 4, 1>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
+        if (packs >= 8 && packs % 2 == 0)
+          return embed_run<Tok, TI, TO, N, 2, 2>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
+        return embed_run<Tok, TI, TO, N, 1, 4>(t, n, e, ld_table, vocab, d, scale, o, ld_out, st);
       });
     });
   });
@@ -170,6 +129,7 @@ constexpr int kSumThreads = 256;
 constexpr int kSumChunk = 1024;    // positions of a piece in shared memory at once
 constexpr int kMaxPieces = 256;    // of one token: what its last block adds up
 constexpr int kSmallRows = 4096;   // up to here one kernel does all
+constexpr int kSmallPacks = 16;
 
 struct GradPlan {
   int tiles, tile;                 // tiles of the sort, tokens of a tile
@@ -489,8 +449,9 @@ embed_sum_kernel(const TG* __restrict__ dout, long long ld, int d, int per_row, 
   }
 }
 
-// Few rows: one kernel.  A block takes `per` tokens and up to 32 packs of
-// columns; it reads all tokens into shared memory, and for each of its own
+// Few rows: one kernel instead of four (4096 x 256: 11 us against 41 us; when
+// all are the same token 40 us against 44 us).  A block takes `per` tokens and up to kSmallPacks packs
+// of columns; it reads all tokens into shared memory, and for each of its own
 // tokens lists the positions in order (a lane keeps the match mask of every
 // 32 positions of its warp's part) and sums their rows.
 template <typename Tok, typename TG, typename TD, int N>
@@ -502,7 +463,7 @@ embed_small_kernel(const Tok* __restrict__ tok, int n, const TG* __restrict__ do
   __shared__ int s_count[kSumThreads / 32];
   __shared__ float s_sum[kSumThreads * N];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int q = d / N, c0 = blockIdx.y * 32, packs = min(32, q - c0);
+  const int q = d / N, c0 = blockIdx.y * kSmallPacks, packs = min(kSmallPacks, q - c0);
 #pragma unroll 8
   for (int i = threadIdx.x; i < n; i += kSumThreads) s_tok[i] = (short)token_index(tok[i], vocab);
   __syncthreads();
@@ -564,7 +525,7 @@ static cudaError_t grad_run(const Tok* tok, long long n, const TG* dout, long lo
   const int q = d / N;
   if (n <= kSmallRows) {
     const int per = (vocab + 147) / 148;
-    embed_small_kernel<Tok, TG, TD, N><<<dim3((vocab + per - 1) / per, (q + 31) / 32), kSumThreads, 0, st>>>(
+    embed_small_kernel<Tok, TG, TD, N><<<dim3((vocab + per - 1) / per, (q + kSmallPacks - 1) / kSmallPacks), kSumThreads, 0, st>>>(
         tok, (int)n, dout, ld, vocab, d, per, scale, accumulate ? 1 : 0, dtable, ld_dtable);
     return cudaGetLastError();
   }
