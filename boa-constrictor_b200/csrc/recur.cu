@@ -26,6 +26,13 @@
 // maps before it applied in order, and the outputs come from the registers.
 // So the gates are read once, nothing waits on another block outside its
 // cluster, and the result does not depend on timing.
+//
+// Measured on a B200 (floor: the bytes at the 6561 GB/s of a copy).  Many 32-bit
+// chains run at the memory's rate: 256 x 1024 x 256 forward 143 us (0.86),
+// backward 243 us (0.84).  16-bit rows are paced by instruction issue, 35 a value
+// forward and 62 backward: 64 x 4096 x 256 bf16 102 us (0.60) and 166 us (0.61).
+// Few chains are paced by the SMs that clusters reach: 1 x 262144 x 512 fp32
+// 500 us (0.49).  One position, 16384 x 256: 13.8 us (0.93).
 #include "kernels.cuh"
 #include "ptx.cuh"
 #include "train_ops.cuh"
@@ -33,7 +40,7 @@
 namespace boa {
 
 constexpr int kSpan = 32;         // positions between two saved states
-constexpr int kMaxWarps = 16;    // warps of a block
+constexpr int kMaxWarps = 16;     // warps of a block
 constexpr int kMaxCluster = 8;    // blocks of a cluster (the portable limit)
 constexpr int kFew = 8;           // up to here, one thread takes a chain through all positions
 // Positions that a warp holds, and registers a thread, for V chains a lane.

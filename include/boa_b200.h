@@ -294,7 +294,9 @@ int boa_embed_backward(const void* d_tokens, int token_type, int64_t n, const vo
  * be NULL; may be d_h0) receives the state after the last position.  With
  * T = 1 this is the decode step.  d_states, when not NULL, receives
  * boa_mingru_states_floats floats that the backward call needs; their layout
- * is the library's own.  T = 0 only moves the state. */
+ * is the library's own.  T = 0 only moves the state.  A gate logit below -88
+ * counts as closed (z = 0); NaN in a row makes the chain's states from there
+ * on, and its gradients, NaN. */
 uint64_t boa_mingru_states_floats(int n_chunks, int T, int d);
 int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
                     const int32_t* d_lengths, const float* d_h0, void* d_h, int64_t h_row, int64_t h_chunk,
