@@ -103,6 +103,21 @@ def test_embed_takes_tokens_of_any_shape(tr):
     assert torch.equal(tr.embed(tok[0, 0, 0], E), E[tok[0, 0, 0]])
 
 
+@pytest.mark.parametrize("d", [4096, 65535, 65536])
+def test_embed_widest_rows(tr, d):
+    import torch
+    tok, E = torch.tensor([3, 0, -1, 3], device="cuda"), torch.randn(4, d, device="cuda")
+    out = tr.embed(tok, E, scale=2.0)
+    assert torch.equal(out[[0, 1, 3]], 2 * E[[3, 0, 3]]) and (out[2] == 0).all()
+    g = torch.randint(-8, 8, (4, d), device="cuda").float()
+    ref = torch.zeros(4, d, device="cuda")
+    ref[0], ref[3] = g[1], g[0] + g[3]
+    assert torch.equal(tr.embed_backward(tok, g, 4), ref)
+    many = torch.arange(6000, device="cuda") % 4
+    g = torch.ones((), device="cuda").expand(6000, d // 16)
+    assert (tr.embed_backward(many, g, 4) == 1500).all()
+
+
 def test_embed_padding_reads_nothing(tr):
     """NaN in the table does not reach padded rows."""
     import torch
@@ -126,6 +141,29 @@ def test_embed_backward(tr, dout_t, dtable_t, n, d, vocab, tok, skew):
     ref, err = R.embed_grad(t, _n(g), vocab, 2.5)
     _close(out, ref, err, dtable_t)
     assert torch.equal(out, tr.embed_backward(tt, g, vocab, scale=2.5, dtype=getattr(torch, dtable_t)))
+
+
+@pytest.mark.parametrize("n,d,vocab,dout_t,skew", [
+    (9000, 5, 1, "float32", False),          # one token, 71 pieces
+    (40000, 12, 3, "bfloat16", True),        # more pieces than are kept of one token
+    (300000, 7, 3, "float32", True),         # pieces longer than a block lists at once
+    (300000, 300, 2, "float16", True),       # and columns in two rounds
+    (5000, 2052, 256, "float32", False), (4096, 300, 1024, "bfloat16", True), (4097, 8, 1024, "float16", False)])
+def test_embed_backward_pieces(tr, n, d, vocab, dout_t, skew):
+    """Long pieces, many pieces and wide rows; the sums in 64 bits by torch."""
+    import torch
+    rng = np.random.default_rng(n + d)
+    t, tt = _tokens(torch, rng, n, vocab, "int32", skew=skew)
+    g = torch.randn(n, d, generator=torch.Generator(device="cuda").manual_seed(d), device="cuda")
+    g = g.to(getattr(torch, dout_t))
+    got = tr.embed_backward(tt, g, vocab)
+    ok = (tt >= 0) & (tt < vocab)
+    ref, size = (torch.zeros(vocab, d, dtype=torch.float64, device="cuda") for _ in range(2))
+    ref.index_add_(0, tt[ok].long(), g[ok].double())
+    size.index_add_(0, tt[ok].long(), g[ok].double().abs())
+    # a piece has at most n / 256 + 128 rows, a token at most 256 pieces, a block at most 256 partial sums
+    err = (n // 256 + 128 + 512) * R.U * _n(size)
+    _close(got, _n(ref), err, "float32")
 
 
 @pytest.mark.parametrize("gap,offset", [(0, 1), (3, 0), (8, 4)])
@@ -213,6 +251,25 @@ def _check_scan(tr, torch, zh, h0, n, dh, dl, dtype):
 def test_mingru(tr, dtype, B, T, d):
     import torch
     _check_scan(tr, torch, *_case(torch, np.random.default_rng(B * T + d), B, T, d, dtype), dtype)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,T,d", [(150, 70, 64), (150, 9, 66), (80, 200, 130), (40, 140, 256), (300, 33, 33)])
+def test_mingru_many_chains(tr, dtype, B, T, d):
+    """Enough chains for several blocks per SM, aligned and not."""
+    import torch
+    lengths = np.random.default_rng(B).integers(0, T + 1, B)
+    lengths[: B // 2] = T
+    _check_scan(tr, torch, *_case(torch, np.random.default_rng(T), B, T, d, dtype, lengths), dtype)
+
+
+def test_mingru_shared_gates(tr):
+    """One chunk's gates expanded over the batch (a stride of 0)."""
+    import torch
+    zh, _, _, dh, dl = _case(torch, np.random.default_rng(12), 1, 300, 32, "float32")
+    zh, dh, dl = zh.expand(5, 300, 64), dh.expand(5, 300, 32), dl.expand(5, 32)
+    h0 = torch.randn(5, 32, device="cuda")
+    _check_scan(tr, torch, zh, h0, None, dh, dl, "float32")
 
 
 @pytest.mark.parametrize("dtype", DT)
@@ -396,6 +453,21 @@ def test_token_loss_nan_and_padding(tr):
     assert torch.isfinite(loss[0]) and torch.isfinite(grad[0]).all()
     assert torch.isnan(loss[1:3]).all() and torch.isnan(grad[1:3]).all()
     assert (loss[3:] == 0).all() and (grad[3:] == 0).all()
+
+
+def test_token_loss_of_one_row_and_of_any_shape(tr):
+    import torch
+    x, t = torch.randn(2, 3, 256, device="cuda"), torch.randint(0, 256, (2, 3), device="cuda")
+    loss, grad = tr.token_loss(x, t, grad_scale=2.0)
+    flat = tr.token_loss(x.view(6, 256), t.view(6), grad_scale=2.0)
+    assert torch.equal(loss.view(6), flat[0]) and torch.equal(grad.view(6, 256), flat[1])
+    one = tr.token_loss(x[0, 0], t[0, 0], grad_scale=2.0)
+    assert one[0].shape == () and torch.equal(one[0], loss[0, 0]) and torch.equal(one[1], grad[0, 0])
+    # logits whose rows no stride reaches are copied; dloss expanded
+    tt = tr.token_loss(x.transpose(0, 1), t.transpose(0, 1), grad_scale=2.0)
+    assert torch.equal(tt[0], loss.t()) and torch.equal(tt[1], grad.transpose(0, 1))
+    half = tr.token_loss(x, t, dloss=torch.full((), 2.0, device="cuda").expand(2, 3))
+    assert torch.equal(half[1], grad)
 
 
 def test_token_loss_empty(tr):
