@@ -16,23 +16,24 @@
 //
 // Both directions are linear in what they carry: over a run of positions the
 // state goes from x to A x + B, with A the product of the run's a.  A group is
-// 32 * V chains (a chain is one channel of one chunk) and is taken along the
+// G * V chains (a chain is one channel of one chunk) and is taken along the
 // time axis by one block, or by a cluster of up to kMaxCluster blocks when
-// there are too few groups to fill the GPU.  In a step of the walk every warp
-// holds P positions of every chain in registers, forms their (A, B), and
-// issues the loads of its next step; the warps' maps meet in shared memory,
+// there are too few groups to fill the GPU.  A team of G lanes (a warp, or half
+// of one where groups are few) has V chains a lane.  In a step of the walk every
+// team holds P positions of every chain in registers, forms their (A, B), and
+// issues the loads of its next step; the teams' maps meet in shared memory,
 // the blocks' in each other's (pushed there, double-buffered, one barrier a
-// step); the state that enters a warp's positions is the walk's state with the
+// step); the state that enters a team's positions is the walk's state with the
 // maps before it applied in order, and the outputs come from the registers.
 // So the gates are read once, nothing waits on another block outside its
 // cluster, and the result does not depend on timing.
 //
 // Measured on a B200 (floor: the bytes at the 6561 GB/s of a copy).  Many 32-bit
-// chains run at the memory's rate: 256 x 1024 x 256 forward 143 us (0.86),
-// backward 243 us (0.84).  16-bit rows are paced by instruction issue, 35 a value
+// chains run at the memory's rate: 256 x 1024 x 256 forward 146 us (0.84),
+// backward 247 us (0.83).  16-bit rows are paced by instruction issue, 35 a value
 // forward and 62 backward: 64 x 4096 x 256 bf16 102 us (0.60) and 166 us (0.61).
 // Few chains are paced by the SMs that clusters reach: 1 x 262144 x 512 fp32
-// 500 us (0.49).  One position, 16384 x 256: 13.8 us (0.93).
+// 392 us (0.63) and 673 us (0.61).  One position, 16384 x 256: 13.8 us (0.93).
 #include "kernels.cuh"
 #include "ptx.cuh"
 #include "train_ops.cuh"
@@ -40,7 +41,6 @@
 namespace boa {
 
 constexpr int kSpan = 32;         // positions between two saved states
-constexpr int kMaxWarps = 16;     // warps of a block
 constexpr int kMaxCluster = 8;    // blocks of a cluster (the portable limit)
 constexpr int kFew = 8;           // up to here, one thread takes a chain through all positions
 // Positions that a warp holds, and registers a thread, for V chains a lane.
@@ -48,14 +48,21 @@ constexpr int kFew = 8;           // up to here, one thread takes a chain throug
 // positions, which is what paces 16-bit rows and few chains (32 x 4096 x 256
 // bf16 forward: 8 positions at 80 registers 69 us, 16 at 128 60 us).  With many
 // 32-bit chains there are bytes enough to wait for, and more warps win
-// (256 x 1024 x 256 forward: 4 positions at 56 registers 143 us, 8 at 80
+// (256 x 1024 x 256 forward: 4 positions at 64 registers 146 us, 8 at 80
 // 169 us).  Backward a position holds twice the values (8 at 128: 95 us, 4 at
 // 80: 134 us).
 template <typename T_, int V>
 constexpr int scan_steps() { return V == 2 && sizeof(T_) == 4 ? 4 : 16; }
 template <typename T_, int V>
-constexpr int scan_regs() { return V == 1 ? 96 : sizeof(T_) == 4 ? 56 : 128; }
-constexpr int kGradSteps = 8, kGradRegs = 128;
+constexpr int scan_regs() { return V == 1 ? 96 : sizeof(T_) == 4 ? 64 : 128; }
+constexpr int kGradSteps = 8;
+template <int V>
+constexpr int grad_regs() { return V == 1 ? 96 : 128; }
+// Warps of a block that has an SM to itself (as many as those registers let
+// in); of the blocks that share one, half of 16.
+template <int V>
+constexpr int alone_warps() { return V == 1 ? 20 : 16; }
+constexpr int kSharedWarps = 8;
 
 // n / d for n < 2^31 by a multiplication: with 2^(s-1) < d <= 2^s and
 // mul = floor(2^(31+s) / d) + 1, mul d exceeds 2^(31+s) by at most d, and
@@ -158,28 +165,28 @@ __device__ __forceinline__ Map<V> then(const Map<V>& m, const Map<V>& n) {
   return {vmul(m.A, n.A), vfma(n.A, m.B, n.B)};
 }
 
-// Shared memory of a walk, for a block of `warps` warps.  Everything is
+// Shared memory of a walk, for a block of `teams` teams.  Everything is
 // double-buffered by the step's parity: what a step writes was last read two
 // steps ago, and every warp passes one barrier in between.
-template <int V>
+template <int V, int G>
 struct Walk {
-  Map<V>* maps;     // [2][warps][32]: the warps' maps
-  Map<V>* forward;  // [2][warps][32]: backward, their maps of the state
-  Map<V>* block;    // [2][ranks][32]: the cluster's blocks' maps, pushed by their owners (ranks > 1)
-  Vec<V>* state;    // [2][32]: the walk's state, left by the last warp (ranks = 1)
+  Map<V>* maps;     // [2][teams][G]: the teams' maps
+  Map<V>* forward;  // [2][teams][G]: backward, their maps of the state
+  Map<V>* block;    // [2][ranks][G]: the cluster's blocks' maps, pushed by their owners (ranks > 1)
+  Vec<V>* state;    // [2][G]: the walk's state, left by the last team (ranks = 1)
   uint64_t* full;   // [2]: barriers that count the bytes pushed into `block` (ranks > 1)
   uint8_t* stages;
-  int warps, ranks;
-  __device__ __forceinline__ Walk(uint8_t* at, int ranks_, bool both) : warps(blockDim.x >> 5), ranks(ranks_) {
+  int teams, ranks;
+  __device__ __forceinline__ Walk(uint8_t* at, int ranks_, bool both) : teams(blockDim.x / G), ranks(ranks_) {
     maps = reinterpret_cast<Map<V>*>(at);
-    forward = maps + 64 * warps;
-    block = forward + (both ? 64 * warps : 0);
-    state = reinterpret_cast<Vec<V>*>(block + (ranks > 1 ? 64 * ranks : 0));
-    full = reinterpret_cast<uint64_t*>(state + 64);
+    forward = maps + 2 * G * teams;
+    block = forward + (both ? 2 * G * teams : 0);
+    state = reinterpret_cast<Vec<V>*>(block + (ranks > 1 ? 2 * G * ranks : 0));
+    full = reinterpret_cast<uint64_t*>(state + 2 * G);
     stages = reinterpret_cast<uint8_t*>(full + 2);
   }
-  static size_t bytes(int warps, int ranks, bool both) {
-    return sizeof(Map<V>) * 64 * ((both ? 2 : 1) * warps + (ranks > 1 ? ranks : 0)) + sizeof(Vec<V>) * 64 + 16;
+  static size_t bytes(int threads, int ranks, bool both) {
+    return sizeof(Map<V>) * 2 * ((both ? 2 : 1) * threads + (ranks > 1 ? ranks * G : 0)) + sizeof(Vec<V>) * 2 * G + 16;
   }
   // Called by all threads before anything else; afterwards the cluster's
   // blocks have started and their barriers are ready.
@@ -198,27 +205,27 @@ struct Walk {
   }
 };
 
-// Where a warp works.  A block's warps form groups of `warps` (a power of
-// two); more than one group per block only when a group's whole sequence fits
-// its warps.
+// Where a team works.  A block serves one group of chains with all its teams,
+// or several groups with `teams` teams each when a group's whole sequence fits
+// them.
 struct Place {
   long long chain;
   bool in;
-  int b, c, lane, warp, warps, first;  // warp within its group, the group's first warp
+  int b, c, lane, team, teams, first;  // lane within the team, team within its group, the group's first team
   int rank, ranks;                     // block within its cluster
 };
-template <int V>
-__device__ __forceinline__ Place place_of(int warps, int ranks, long long chains, int d, FastDiv by_d) {
+template <int V, int G>
+__device__ __forceinline__ Place place_of(int teams, int ranks, long long chains, int d, FastDiv by_d) {
   Place p;
-  p.lane = threadIdx.x & 31;
-  const int w = threadIdx.x >> 5, per = (int)(blockDim.x >> 5) / warps;
-  p.warps = warps;
-  p.warp = w % warps;
-  p.first = w - p.warp;
+  p.lane = threadIdx.x % G;
+  const int w = threadIdx.x / G, per = (int)(blockDim.x / G) / teams;
+  p.teams = teams;
+  p.team = w % teams;
+  p.first = w - p.team;
   p.ranks = ranks;
   p.rank = ranks > 1 ? (int)cluster_rank() : 0;
-  const long long group = (long long)(blockIdx.x / ranks) * per + w / warps;
-  p.chain = group * (32 * V) + p.lane * V;
+  const long long group = (long long)(blockIdx.x / ranks) * per + w / teams;
+  p.chain = group * (G * V) + p.lane * V;
   p.in = p.chain < chains;
   p.b = p.in ? (int)div_by((uint32_t)p.chain, by_d) : 0;
   p.c = p.in ? (int)(p.chain - (long long)p.b * d) : 0;
@@ -251,72 +258,69 @@ __device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) 
       : "memory");
   return ok != 0;
 }
-// false when the wait ran out: the walk's state is then NaN, and the walk goes
-// on without waiting again (a handle-free call has no error word to set)
-__device__ __forceinline__ bool await_maps(uint32_t bar, uint32_t parity) {
-  bool there = try_wait_cluster(bar, parity);
-  if (!there) {
+// Waits for a phase.  When the wait runs out `waiting` is cleared: the walk's
+// state becomes NaN, and the walk goes on without waiting again (a handle-free
+// call has no error word to set).
+__device__ __forceinline__ void await_maps(uint32_t bar, uint32_t parity, bool& waiting) {
+  if (waiting && !try_wait_cluster(bar, parity)) {
     const uint64_t t0 = global_ns();
-    while (!(there = try_wait_cluster(bar, parity)) && global_ns() - t0 <= kWaitLimitNs) {}
+    while (waiting && !try_wait_cluster(bar, parity)) waiting = global_ns() - t0 <= kWaitLimitNs;
   }
   __syncwarp();  // lanes may leave the loop apart
-  return there;
 }
 
-// One step's exchange.  `mine`: the map of this warp's positions, `x`: the
-// walk's state before the step.  Returns the state before this warp's
+// One step's exchange.  `mine`: the map of this team's positions, `x`: the
+// walk's state before the step.  Returns the state before this team's
 // positions; in a cluster x becomes the state after the step.  REVERSE runs
-// from the last warp and block to the first.  Without a cluster the state
+// from the last team and block to the first.  Without a cluster the state
 // after the step is handed on through leave().
 //
 // In a cluster, a slot of `block` is written again two steps on.  Its writer
 // has then seen this block's map of the step between, which goes out after
-// the barrier below, that is after all warps here have read the slot.
-template <int V, bool REVERSE>
-__device__ __forceinline__ Vec<V> exchange(const Walk<V>& K, const Place& p, int step, const Map<V>& mine, Vec<V>& x,
-                                           bool& waiting) {
+// the barrier below, that is after all teams here have read the slot.
+template <int V, int G, bool REVERSE>
+__device__ __forceinline__ Vec<V> exchange(const Walk<V, G>& K, const Place& p, int step, const Map<V>& mine,
+                                           Vec<V>& x, bool& waiting) {
   const int parity = step & 1;
-  const int order = REVERSE ? p.warps - 1 - p.warp : p.warp;  // place of this warp along the walk
-  Map<V>* maps = K.maps + (parity * K.warps + p.first) * 32 + p.lane;
-  maps[order * 32] = mine;
+  const int order = REVERSE ? p.teams - 1 - p.team : p.team;  // place of this team along the walk
+  Map<V>* maps = K.maps + (parity * K.teams + p.first) * G + p.lane;
+  maps[order * G] = mine;
   __syncthreads();
   Vec<V> s;
   if (p.ranks == 1) {
-    s = step == 0 ? x : K.state[parity * 32 + p.lane];
+    s = step == 0 ? x : K.state[parity * G + p.lane];
   } else {
-    const uint32_t bar = smem_u32(K.full + parity);
-    if (threadIdx.x == 0) mbar_arrive_expect_tx(K.full + parity, (uint32_t)(p.ranks * 32 * sizeof(Map<V>)));
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(K.full + parity, (uint32_t)(p.ranks * G * sizeof(Map<V>)));
     const int turn = REVERSE ? p.ranks - 1 - p.rank : p.rank;
-    if (p.warp < p.ranks) {  // warp r takes the block's map to block r
+    if (p.team < p.ranks) {  // team r takes the block's map to block r
       Map<V> all = maps[0];
-      for (int w = 1; w < p.warps; ++w) all = then<V>(all, maps[w * 32]);
-      push_map<V>(cluster_addr(K.block + (parity * p.ranks + turn) * 32 + p.lane, (uint32_t)p.warp), all,
-                  cluster_addr(K.full + parity, (uint32_t)p.warp));
+#pragma unroll 4
+      for (int w = 1; w < p.teams; ++w) all = then<V>(all, maps[w * G]);
+      push_map<V>(cluster_addr(K.block + (parity * p.ranks + turn) * G + p.lane, (uint32_t)p.team), all,
+                  cluster_addr(K.full + parity, (uint32_t)p.team));
     }
-    if (waiting && !await_maps(bar, (uint32_t)(step >> 1) & 1u)) {
-      waiting = false;
-      x = all_of<V>(__int_as_float(0x7fffffff));
-    }
+    await_maps(smem_u32(K.full + parity), (uint32_t)(step >> 1) & 1u, waiting);
+    if (!waiting) x = all_of<V>(__int_as_float(0x7fffffff));
     for (int r = 0; r < p.ranks; ++r) {
       if (r == turn) s = x;
-      x = apply<V>(K.block[(parity * p.ranks + r) * 32 + p.lane], x);
+      x = apply<V>(K.block[(parity * p.ranks + r) * G + p.lane], x);
     }
   }
 #pragma unroll 4
-  for (int w = 0; w < order; ++w) s = apply<V>(maps[w * 32], s);
+  for (int w = 0; w < order; ++w) s = apply<V>(maps[w * G], s);
   return s;
 }
 // The state after the step, for the next one (no cluster): the group's last
-// warp along the walk has it.
-template <int V, bool REVERSE>
-__device__ __forceinline__ void leave(const Walk<V>& K, const Place& p, int parity, const Vec<V>& s) {
-  if (p.ranks == 1 && (REVERSE ? p.warp == 0 : p.warp == p.warps - 1)) K.state[(parity ^ 1) * 32 + p.lane] = s;
+// team along the walk has it.
+template <int V, int G, bool REVERSE>
+__device__ __forceinline__ void leave(const Walk<V, G>& K, const Place& p, int parity, const Vec<V>& s) {
+  if (p.ranks == 1 && (REVERSE ? p.team == 0 : p.team == p.teams - 1)) K.state[(parity ^ 1) * G + p.lane] = s;
 }
 
-// Rows on their way from HBM to a warp's stage, [row][32 lanes] packs a
+// Rows on their way from HBM to a team's stage, [row][G lanes] packs a
 // stream.  QUADS: 16 bytes a lane, several rows an instruction, where every
 // row lets them be moved whole (a lane then brings packs that other lanes of
-// its warp use).  Otherwise every lane brings its own packs; one of 2 bytes
+// its team use).  Otherwise every lane brings its own packs; one of 2 bytes
 // (odd widths) is too small for an asynchronous copy and is moved by a load
 // and a store.
 template <int BYTES>
@@ -355,10 +359,15 @@ __device__ __forceinline__ void store_rounded(T_* to, const Vec<V>& x) {
   *reinterpret_cast<Pack<T_, V>*>(to) = narrow_pack<T_>(x.v);
 }
 
-// A warp's stages, [stage][stream][P][32].
-template <typename T_, int V, int P, int STREAMS>
-__device__ __forceinline__ Pack<T_, V>* warp_stages(uint8_t* stages, int S) {
-  return reinterpret_cast<Pack<T_, V>*>(stages) + (threadIdx.x >> 5) * (S * STREAMS * P * 32);
+// A team's stages, [stage][stream][P][G].  Half-warp teams lie half the banks
+// apart, so that the two of a warp read without conflicts.
+template <int G>
+__host__ __device__ constexpr int packs_of_team(int stages, int streams, int P) {
+  return stages * streams * P * G + (G == 32 ? 0 : G);
+}
+template <typename T_, int V, int G, int P, int STREAMS>
+__device__ __forceinline__ Pack<T_, V>* team_stages(uint8_t* stages, int S) {
+  return reinterpret_cast<Pack<T_, V>*>(stages) + (threadIdx.x / G) * packs_of_team<G>(S, STREAMS, P);
 }
 // row p after `x`, `row` bytes each: one multiply-add of 32 bits to 64
 template <typename P_>
@@ -366,18 +375,18 @@ __device__ __forceinline__ P_* row_at(P_* x, uint32_t row, int p) {
   using B_ = typename std::conditional<std::is_const<P_>::value, const char, char>::type;
   return reinterpret_cast<P_*>(reinterpret_cast<B_*>(x) + (unsigned long long)row * (uint32_t)p);
 }
-// Which part of a warp's rows a lane brings: elements `c` on of chunk `b`, of
+// Which part of a team's rows a lane brings: elements `c` on of chunk `b`, of
 // rows first, first + EVERY, ...; `at` bytes into the stage.
-template <typename T_, int V, bool QUADS>
+template <typename T_, int V, int G, bool QUADS>
 struct Carrier {
   static constexpr int kBytes = QUADS ? 16 : (int)sizeof(T_) * V;
-  static constexpr int kRow = 32 * (int)sizeof(T_) * V;      // bytes of a row in the stage
-  static constexpr int kEvery = 32 * kBytes / kRow;          // rows of an instruction
+  static constexpr int kRow = G * (int)sizeof(T_) * V;       // bytes of a row in the stage
+  static constexpr int kEvery = G * kBytes / kRow;           // rows of an instruction
   int b, c, first, len;
   uint32_t at;
   __device__ __forceinline__ Carrier(const Place& p, int T, int d, FastDiv by_d, long long chains, const int* lengths) {
-    const int piece = p.lane % (32 / kEvery);
-    first = p.lane / (32 / kEvery);
+    const int piece = p.lane % (G / kEvery);
+    first = p.lane / (G / kEvery);
     at = (uint32_t)(p.lane * kBytes);
     const long long chain = p.chain - p.lane * V + piece * (kBytes / (int)sizeof(T_));
     const bool in = chain < chains;
@@ -409,38 +418,40 @@ constexpr int kStages = 2;  // the step in use, and the next one on its way
 
 // Positions that are not a chunk's get a gate logit of -inf: a = 1 and b = 0
 // exactly, which leaves the state alone.  (p r = 0 there, and so is f (p r).)
-// A warp whose rows are all there (`whole`, the same for its lanes) takes a
-// form without those tests.
+// A warp whose rows are all there (`whole`, the same for its lanes: `later` is
+// how much later its last team's positions begin) takes a form without those
+// tests.
 // ------------------------------------------------------------------ forward
-template <typename T_, int V, bool QUADS>
+template <typename T_, int V, int G, bool QUADS>
 __global__ void __maxnreg__((scan_regs<T_, V>()))
 mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains,
                    const int* __restrict__ lengths, const float* h0, T_* __restrict__ h, RowStrides hs,
-                   float* h_last, float* __restrict__ states, int warps, int ranks) {
-  constexpr int P = scan_steps<T_, V>(), S = kStages, STAGE = 2 * P * 32;
+                   float* h_last, float* __restrict__ states, int teams, int ranks) {
+  constexpr int P = scan_steps<T_, V>(), S = kStages, STAGE = 2 * P * G;
   extern __shared__ __align__(16) uint8_t walk_smem[];
-  const Walk<V> K(walk_smem, ranks, false);
+  const Walk<V, G> K(walk_smem, ranks, false);
   K.start();
-  const Place at = place_of<V>(warps, ranks, chains, d, by_d);
+  const Place at = place_of<V, G>(teams, ranks, chains, d, by_d);
   int len = at.in ? T : 0;
   if (at.in && lengths) len = min(max(lengths[at.b], 0), T);
   const int end = at.in ? T : 0;
   const int all_len = __reduce_min_sync(~0u, len);  // positions that all of the warp's chains have
-  const int step = ranks * warps * P;  // positions of a step of the walk
-  int t = (at.rank * warps + at.warp) * P;
-  const Carrier<T_, V, QUADS> by(at, T, d, by_d, chains, lengths);
+  const int later = P * ((32 / G - 1) - at.team % (32 / G));
+  const int step = ranks * teams * P;  // positions of a step of the walk
+  int t = (at.rank * teams + at.team) * P;
+  const Carrier<T_, V, G, QUADS> by(at, T, d, by_d, chains, lengths);
   const T_* x = zh + by.b * zs.chunk + (t + by.first) * zs.row + by.c;
   T_* o = h + at.b * hs.chunk + t * hs.row + at.c;
-  Pack<T_, V>* const stages = warp_stages<T_, V, P, 2>(K.stages, S);
+  Pack<T_, V>* const stages = team_stages<T_, V, G, P, 2>(K.stages, S);
   const long long x_step = step * zs.row, o_step = step * hs.row;
   const uint32_t x_row = (uint32_t)(zs.row * sizeof(T_)), o_row = (uint32_t)(hs.row * sizeof(T_));
   const int steps = (T + step - 1) / step;
   int t_next = t, put = 0, got = 0;  // the next step to fetch, its stage, and the stage in use
   auto fetch = [&](bool more) {
     if (more) {
-      const bool whole = t_next + P <= all_len;
+      const bool whole = t_next + later + P <= all_len;
       by.template copy<P>(stages + put * STAGE, x, x_row, t_next, whole);
-      by.template copy<P>(stages + put * STAGE + P * 32, x + d, x_row, t_next, whole);
+      by.template copy<P>(stages + put * STAGE + P * G, x + d, x_row, t_next, whole);
       x += x_step;
       t_next += step;
       put = put + 1 == S ? 0 : put + 1;
@@ -457,10 +468,10 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
   for (int i = 0; i < steps; ++i) {
     copies_wait<S - 2>();
     __syncwarp();  // the other lanes' copies too
-    const Pack<T_, V>*zl = stages + got * STAGE + at.lane, *hr = zl + P * 32;
+    const Pack<T_, V>*zl = stages + got * STAGE + at.lane, *hr = zl + P * G;
     got = got + 1 == S ? 0 : got + 1;
     const int live = rows_left<P>(t, len), rows = rows_left<P>(t, end);
-    const bool whole = t + P <= all_len;
+    const bool whole = t + later + P <= all_len;
     Vec<V> ga[P], gb[P];
     Map<V> m;
     auto gates = [&](auto all) {
@@ -468,8 +479,8 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const bool there = ALL || p < live;
-        const Cell<V> k = mingru_cell<V, false>(widen(zl[p * 32], there, -INFINITY),
-                                                widen(hr[p * 32], there, 0.f));
+        const Cell<V> k = mingru_cell<V, false>(widen(zl[p * G], there, -INFINITY),
+                                                widen(hr[p * G], there, 0.f));
         ga[p] = k.a;
         gb[p] = k.b;
         m = p ? then<V>(m, {k.a, k.b}) : Map<V>{k.a, k.b};
@@ -478,7 +489,7 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     if (whole) gates(std::true_type{});
     else gates(std::false_type{});
     fetch(i + S - 1 < steps);
-    s = exchange<V, false>(K, at, i, m, walk, waiting);
+    s = exchange<V, G, false>(K, at, i, m, walk, waiting);
     if (states && rows > 0 && t % kSpan == 0)
 #pragma unroll
       for (int v = 0; v < V; ++v) states[t / kSpan * chains + at.chain + v] = s.v[v];
@@ -493,40 +504,41 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     };
     if (whole) finish(std::true_type{});
     else finish(std::false_type{});
-    if (i + 1 < steps) leave<V, false>(K, at, i & 1, s);
+    if (i + 1 < steps) leave<V, G, false>(K, at, i & 1, s);
     t += step;
     o += o_step;
   }
-  // the state after the last position: the walk's last warp has applied all
-  if (h_last && at.in && at.rank == ranks - 1 && at.warp == warps - 1)
+  // the state after the last position: the walk's last team has applied all
+  if (h_last && at.in && at.rank == ranks - 1 && at.team == teams - 1)
 #pragma unroll
     for (int v = 0; v < V; ++v) h_last[at.chain + v] = s.v[v];
   K.finish();
 }
 
 // ----------------------------------------------------------------- backward
-template <typename T_, int V, bool QUADS>
-__global__ void __maxnreg__(kGradRegs)
+template <typename T_, int V, int G, bool QUADS>
+__global__ void __maxnreg__(grad_regs<V>())
 mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains,
                    const int* __restrict__ lengths, const float* __restrict__ states, const T_* __restrict__ dh,
-                   RowStrides dhs, const float* dh_last, T_* __restrict__ dzh, RowStrides dzs, float* dh0, int warps,
+                   RowStrides dhs, const float* dh_last, T_* __restrict__ dzh, RowStrides dzs, float* dh0, int teams,
                    int ranks) {
-  constexpr int P = kGradSteps, S = kStages, STAGE = 3 * P * 32;
+  constexpr int P = kGradSteps, S = kStages, STAGE = 3 * P * G;
   extern __shared__ __align__(16) uint8_t walk_smem[];
-  const Walk<V> K(walk_smem, ranks, true);
+  const Walk<V, G> K(walk_smem, ranks, true);
   K.start();
-  const Place at = place_of<V>(warps, ranks, chains, d, by_d);
+  const Place at = place_of<V, G>(teams, ranks, chains, d, by_d);
   int len = at.in ? T : 0;
   if (at.in && lengths) len = min(max(lengths[at.b], 0), T);
   const int end = at.in ? T : 0;
   const int all_len = __reduce_min_sync(~0u, len);  // positions that all of the warp's chains have
-  const int step = ranks * warps * P;
+  const int later = P * ((32 / G - 1) - at.team % (32 / G));
+  const int step = ranks * teams * P;
   const int steps = (T + step - 1) / step;
   // steps are taken from the last
-  int t = (steps - 1) * step + (at.rank * warps + at.warp) * P;
-  // the warps between the saved state and this warp's positions
-  const int lead = at.warp % min(warps, kSpan / P);
-  const Carrier<T_, V, QUADS> by(at, T, d, by_d, chains, lengths);
+  int t = (steps - 1) * step + (at.rank * teams + at.team) * P;
+  // the teams between the saved state and this team's positions
+  const int lead = at.team % min(teams, kSpan / P);
+  const Carrier<T_, V, G, QUADS> by(at, T, d, by_d, chains, lengths);
   const T_* x = zh + by.b * zs.chunk + (t + by.first) * zs.row + by.c;
   const T_* u = dh + by.b * dhs.chunk + (t + by.first) * dhs.row + by.c;
   T_* o = dzh + at.b * dzs.chunk + t * dzs.row + at.c;
@@ -534,14 +546,14 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
   const uint32_t x_row = (uint32_t)(zs.row * sizeof(T_)), u_row = (uint32_t)(dhs.row * sizeof(T_)),
                  o_row = (uint32_t)(dzs.row * sizeof(T_));
   Vec<V> next_saved = all_of<V>(0.f);  // the saved state of the step after the current one
-  Pack<T_, V>* const stages = warp_stages<T_, V, P, 3>(K.stages, S);
+  Pack<T_, V>* const stages = team_stages<T_, V, G, P, 3>(K.stages, S);
   int t_next = t, put = 0, got = 0;  // the next step to fetch, its stage, and the stage in use
   auto fetch = [&](bool more) {
     if (more) {
-      const bool whole = t_next + P <= all_len;
+      const bool whole = t_next + later + P <= all_len;
       by.template copy<P>(stages + put * STAGE, x, x_row, t_next, whole);
-      by.template copy<P>(stages + put * STAGE + P * 32, x + d, x_row, t_next, whole);
-      by.template copy<P>(stages + put * STAGE + 2 * P * 32, u, u_row, t_next, whole);
+      by.template copy<P>(stages + put * STAGE + P * G, x + d, x_row, t_next, whole);
+      by.template copy<P>(stages + put * STAGE + 2 * P * G, u, u_row, t_next, whole);
       x -= x_step;
       u -= u_step;
       t_next -= step;
@@ -565,12 +577,12 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
   for (int i = 0; i < steps; ++i) {
     copies_wait<S - 2>();
     __syncwarp();  // the other lanes' copies too, and all have read the stage that is filled next
-    const Pack<T_, V>*zl = stages + got * STAGE + at.lane, *hr = zl + P * 32, *du = hr + P * 32;
+    const Pack<T_, V>*zl = stages + got * STAGE + at.lane, *hr = zl + P * G, *du = hr + P * G;
     got = got + 1 == S ? 0 : got + 1;
     const int live = rows_left<P>(t, len), rows = rows_left<P>(t, end);
     Vec<V> s = next_saved;
     if (i + 1 < steps) load_saved(t - step);
-    const bool whole = t + P <= all_len;
+    const bool whole = t + later + P <= all_len;
     Vec<V> ga[P], gb[P], gz[P], gw[P];
     Map<V> m, r;
     auto gates = [&](auto all) {
@@ -578,8 +590,8 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
 #pragma unroll
       for (int p = 0; p < P; ++p) {
         const bool there = ALL || p < live;
-        const Cell<V> k = mingru_cell<V, true>(widen(zl[p * 32], there, -INFINITY),
-                                               widen(hr[p * 32], there, 0.f));
+        const Cell<V> k = mingru_cell<V, true>(widen(zl[p * G], there, -INFINITY),
+                                               widen(hr[p * G], there, 0.f));
         ga[p] = k.a;
         gb[p] = k.b;
         gz[p] = k.z;
@@ -591,16 +603,16 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     else gates(std::false_type{});
     // the gradient that reaches each state: G_p = u_p + a_{p+1} G_{p+1}
     r.A = m.A;
-    r.B = widen(du[(P - 1) * 32], P - 1 < live, 0.f);
+    r.B = widen(du[(P - 1) * G], P - 1 < live, 0.f);
 #pragma unroll
-    for (int p = P - 2; p >= 0; --p) r.B = vfma(ga[p + 1], r.B, widen(du[p * 32], p < live, 0.f));
+    for (int p = P - 2; p >= 0; --p) r.B = vfma(ga[p + 1], r.B, widen(du[p * G], p < live, 0.f));
     r.B = vmul(ga[0], r.B);
     fetch(i + S - 1 < steps);
-    Map<V>* forward = K.forward + ((i & 1) * K.warps + at.first) * 32 + at.lane;
-    forward[at.warp * 32] = m;
-    g = exchange<V, true>(K, at, i, r, walk, waiting);
+    Map<V>* forward = K.forward + ((i & 1) * K.teams + at.first) * G + at.lane;
+    forward[at.team * G] = m;
+    g = exchange<V, G, true>(K, at, i, r, walk, waiting);
 #pragma unroll 4
-    for (int w = at.warp - lead; w < at.warp; ++w) s = apply<V>(forward[w * 32], s);
+    for (int w = at.team - lead; w < at.team; ++w) s = apply<V>(forward[w * G], s);
     // dzl / G = a (z c - z h'), h' the state before
 #pragma unroll
     for (int p = 0; p < P; ++p) {
@@ -615,7 +627,7 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
 #pragma unroll
       for (int p = P - 1; p >= 0; --p) {
         const bool there = ALL || p < live;
-        const Vec<V> u_p = widen(du[p * 32], there, 0.f);
+        const Vec<V> u_p = widen(du[p * G], there, 0.f);
         g = vfma(p == P - 1 ? all_of<V>(1.f) : ga[p + 1], g, u_p);
         if (ALL || p < rows) {
           T_* y = row_at(o, o_row, p);
@@ -627,11 +639,11 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     };
     if (whole) finish(std::true_type{});
     else finish(std::false_type{});
-    if (i + 1 < steps) leave<V, true>(K, at, i & 1, g);
+    if (i + 1 < steps) leave<V, G, true>(K, at, i & 1, g);
     t -= step;
     o -= o_step;
   }
-  if (dh0 && at.in && at.rank == 0 && at.warp == 0)
+  if (dh0 && at.in && at.rank == 0 && at.team == 0)
 #pragma unroll
     for (int v = 0; v < V; ++v) dh0[at.chain + v] = g.v[v];
   K.finish();
@@ -689,14 +701,15 @@ static bool moved_whole(int n, int d, int type, std::initializer_list<std::pair<
   return true;
 }
 
-// The shape of a walk: warps of a group in a block, blocks of a group, groups
-// of a block.
-struct Shape {
-  int warps, ranks, per;
-};
-// Clusters of `ranks` blocks that the device holds at once.
-template <typename K>
-static int clusters_at_once(K kernel, int ranks, unsigned threads, size_t smem) {
+// Clusters of `ranks` blocks that the device holds at once: a property of the
+// kernel and the device, asked once for each.
+template <auto KERNEL>
+static int clusters_at_once(int ranks, unsigned threads, size_t smem) {
+  static std::atomic<int> known[64][kMaxCluster + 1];  // + 1; 0 = not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  const int k = known[dev][ranks].load(std::memory_order_relaxed);
+  if (k) return k - 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)ranks);
   cfg.blockDim = dim3(threads);
@@ -708,43 +721,59 @@ static int clusters_at_once(K kernel, int ranks, unsigned threads, size_t smem) 
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
+  known[dev][ranks].store(n + 1, std::memory_order_relaxed);
   return n;
 }
-// Launches `kernel` over `chains` chains of T positions, P to a warp;
-// smem(warps, ranks) gives a block's shared memory.
-template <int V, typename K, typename M, typename... A>
-static cudaError_t launch_walk(K kernel, long long chains, int T, int P, M smem, cudaStream_t st, A... args) {
-  const long long groups = (chains + 32 * V - 1) / (32 * V);
-  Shape s{1, 1, 1};
-  const bool dense = groups >= 148;  // enough groups to give every SM blocks of its own
-  const int block_warps = dense ? kMaxWarps / 2 : kMaxWarps;
-  while (s.warps < block_warps && (long long)s.warps * P < T) s.warps *= 2;
-  if (s.warps > block_warps) s.warps = block_warps;
-  if ((long long)s.warps * P >= T) s.per = block_warps / s.warps;
-  const unsigned threads = (unsigned)(s.warps * s.per * 32);
-  size_t bytes = smem((int)threads / 32, kMaxCluster);
+
+// The shape of a walk of T positions, P to a team: teams and blocks of a group,
+// groups of a block, threads and shared memory of a block, and how many SMs
+// have work.
+struct Shape {
+  int teams, ranks, per, threads;
+  size_t smem;
+  long long reach;
+};
+template <auto KERNEL, int V, int G, typename M>
+static cudaError_t shape_of(long long chains, int T, int P, M smem, Shape& s) {
+  const long long groups = (chains + G * V - 1) / (G * V);
+  const bool shared = groups >= 148;  // enough groups to give every SM blocks of its own
+  const int block_teams = (shared ? kSharedWarps : alone_warps<V>()) * (32 / G);
+  s = {1, 1, 1, 0, 0, 0};
+  while (s.teams < block_teams && (long long)s.teams * P < T) s.teams *= 2;
+  if (s.teams > block_teams) s.teams = block_teams;
+  // short sequences: several groups a block, as long as there are two blocks an SM
+  if ((long long)s.teams * P >= T)
+    while (s.per * 2 * s.teams <= block_teams && groups / (s.per * 2) >= 2 * 148) s.per *= 2;
+  s.threads = s.teams * s.per * G;
+  if (s.threads < 32) s.threads = 32;  // two half-warp teams, of two groups
+  if (s.threads > s.teams * s.per * G) s.per = s.threads / (s.teams * G);
+  const size_t most_smem = smem(s.threads, kMaxCluster);
   // clusters are packed: two of their blocks on one SM while another stays
   // empty, unless a block takes more than half of the shared memory
-  const size_t alone = bytes < 116 * 1024 ? 116 * 1024 : bytes;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)alone);
+  const size_t alone = most_smem < 116 * 1024 ? 116 * 1024 : most_smem;
+  const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)alone);
   if (e != cudaSuccess) return e;
-  if (s.per == 1 && groups * 2 <= 148) {
-    int most = kMaxCluster;
-    while (most > 1 && (long long)(most - 1) * s.warps * P >= T) --most;
-    for (int r = most; r > 1; --r)
-      if (groups * r <= 148 && clusters_at_once(kernel, r, threads, alone) >= groups) {
+  if (s.teams == block_teams && groups * 2 <= 148)
+    for (int r = kMaxCluster; r > 1; --r)
+      if ((long long)(r - 1) * s.teams * P < T && groups * r <= 148 &&
+          clusters_at_once<KERNEL>(r, (unsigned)s.threads, alone) >= groups) {
         s.ranks = r;
         break;
       }
-  }
+  s.smem = s.ranks > 1 ? alone : smem(s.threads, 1);
+  s.reach = (groups + s.per - 1) / s.per * s.ranks;
+  return cudaSuccess;
+}
+template <auto KERNEL, typename... A>
+static cudaError_t launch_walk(const Shape& s, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((groups + s.per - 1) / s.per * s.ranks));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = s.ranks > 1 && !dense ? alone : smem((int)threads / 32, s.ranks);
+  cfg.gridDim = dim3((unsigned)s.reach);
+  cfg.blockDim = dim3((unsigned)s.threads);
+  cfg.dynamicSmemBytes = s.smem;
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -752,8 +781,26 @@ static cudaError_t launch_walk(K kernel, long long chains, int T, int P, M smem,
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = s.ranks > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kernel, args..., s.warps, s.ranks);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, KERNEL, args..., s.teams, s.ranks);
   return e != cudaSuccess ? e : cudaGetLastError();
+}
+// Shared memory of a block.
+template <typename E, int V, int G>
+static size_t scan_smem(int threads, int ranks) {
+  return Walk<V, G>::bytes(threads, ranks, false) +
+         (size_t)packs_of_team<G>(kStages, 2, scan_steps<E, V>()) * (threads / G) * sizeof(Pack<E, V>);
+}
+template <typename E, int V, int G>
+static size_t grad_smem(int threads, int ranks) {
+  return Walk<V, G>::bytes(threads, ranks, true) +
+         (size_t)packs_of_team<G>(kStages, 3, kGradSteps) * (threads / G) * sizeof(Pack<E, V>);
+}
+// Half-warp teams make twice the groups.  They are taken where more SMs then
+// have work (1 x 262144 x 512 fp32 forward: 16 clusters of 6, 473 us, against
+// 32 of 4, 392 us; 1 x 65536 x 64: 95 us and 56 us), not where as many have
+// (4 x 16384 x 256: 53 us and 58 us).
+static bool half_reaches_further(const Shape& half, const Shape& warp) {
+  return half.reach <= 148 && half.reach > warp.reach;
 }
 
 cudaError_t launch_mingru_scan(const void* zh, int type, RowStrides zs, int B, int T, int d, const int* lengths,
@@ -780,11 +827,21 @@ cudaError_t launch_mingru_scan(const void* zh, int type, RowStrides zs, int B, i
                                                                        h_last, states);
         return cudaGetLastError();
       }
-      auto smem = [](int w, int ranks) {
-        return Walk<V>::bytes(w, ranks, false) + (size_t)kStages * 2 * scan_steps<E, V>() * w * 32 * sizeof(Pack<E, V>);
-      };
-      return launch_walk<V>(mingru_scan_kernel<E, V, Q>, chains, T, scan_steps<E, V>(), smem, st, x, zs, T, d, by_d, chains,
-                            lengths, h0, o, hs, h_last, states);
+      constexpr auto kernel = mingru_scan_kernel<E, V, 32, Q>;
+      constexpr int P = scan_steps<E, V>();
+      Shape s, n;
+      cudaError_t e = shape_of<kernel, V, 32>(chains, T, P, scan_smem<E, V, 32>, s);
+      if (e != cudaSuccess) return e;
+      if constexpr (Q && !(V == 2 && sizeof(E) == 4)) {  // those have groups enough
+        constexpr auto narrow = mingru_scan_kernel<E, V, 16, Q>;
+        if (s.reach < 148) {
+          e = shape_of<narrow, V, 16>(chains, T, P, scan_smem<E, V, 16>, n);
+          if (e != cudaSuccess) return e;
+          if (half_reaches_further(n, s))
+            return launch_walk<narrow>(n, st, x, zs, T, d, by_d, chains, lengths, h0, o, hs, h_last, states);
+        }
+      }
+      return launch_walk<kernel>(s, st, x, zs, T, d, by_d, chains, lengths, h0, o, hs, h_last, states);
     };
     // two chains a lane: always for 16 bits; for 32 bits where that leaves
     // groups enough to fill the GPU
@@ -810,15 +867,25 @@ cudaError_t launch_mingru_scan_grad(const void* zh, int type, RowStrides zs, int
   const bool quads = moved_whole(16 / type_bytes(type), d, type, {{zh, zs}, {dh, dhs}});
   return with_type(type, [&](auto t) {
     using E = decltype(t);
-    auto go = [&](auto vec, auto whole) {
+    auto go = [&](auto vec, auto whole) -> cudaError_t {
       constexpr int V = decltype(vec)::value;
       constexpr bool Q = decltype(whole)::value;
-      auto smem = [](int w, int ranks) {
-        return Walk<V>::bytes(w, ranks, true) + (size_t)kStages * 3 * kGradSteps * w * 32 * sizeof(Pack<E, V>);
-      };
-      return launch_walk<V>(mingru_grad_kernel<E, V, Q>, chains, T, kGradSteps, smem, st, static_cast<const E*>(zh), zs,
-                            T, d, by_d, chains, lengths, states, static_cast<const E*>(dh), dhs, dh_last,
-                            static_cast<E*>(dzh), dzs, dh0);
+      constexpr auto kernel = mingru_grad_kernel<E, V, 32, Q>;
+      const E *x = static_cast<const E*>(zh), *u = static_cast<const E*>(dh);
+      E* o = static_cast<E*>(dzh);
+      Shape s, n;
+      cudaError_t e = shape_of<kernel, V, 32>(chains, T, kGradSteps, grad_smem<E, V, 32>, s);
+      if (e != cudaSuccess) return e;
+      if constexpr (Q) {
+        constexpr auto narrow = mingru_grad_kernel<E, V, 16, Q>;
+        if (s.reach < 148) {
+          e = shape_of<narrow, V, 16>(chains, T, kGradSteps, grad_smem<E, V, 16>, n);
+          if (e != cudaSuccess) return e;
+          if (half_reaches_further(n, s))
+            return launch_walk<narrow>(n, st, x, zs, T, d, by_d, chains, lengths, states, u, dhs, dh_last, o, dzs, dh0);
+        }
+      }
+      return launch_walk<kernel>(s, st, x, zs, T, d, by_d, chains, lengths, states, u, dhs, dh_last, o, dzs, dh0);
     };
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;

@@ -4,6 +4,7 @@
 // element types; all arithmetic is fp32 or wider, and a result is rounded
 // once, to nearest, when it is stored.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <initializer_list>
 #include <type_traits>
