@@ -352,6 +352,90 @@ embed_order_kernel(const Tok* __restrict__ tok, long long n, int vocab, int tile
   }
 }
 
+// Up to kClusterRows rows: one cluster of eight blocks sorts instead of three
+// launches of the kernels above (the whole gradient of 5000 x 256: 23 us against
+// 35 us, of 20000 x 160 over 1000 tokens 24 and 40; from 65536 rows on the
+// eight SMs are slower, 29.5 and 27.5).  A block counts its eighth of the
+// positions, 32 warps with a row of counts each; the blocks read each other's
+// totals, and go on as above.
+constexpr int kClusterBlocks = 8, kClusterThreads = 1024, kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterHeld = 6;   // tokens of a lane
+constexpr int kClusterRows = kClusterBlocks * kClusterThreads * kClusterHeld;
+
+template <typename Tok>
+__global__ void __launch_bounds__(kClusterThreads)
+embed_sort_kernel(const Tok* __restrict__ tok, int n, int span, int vocab, int rows, Piece* __restrict__ pieces,
+                  int* __restrict__ done, int* __restrict__ order) {
+  // [kClusterWarps][vocab] counts, the block's totals [vocab], first places [vocab], scratch
+  extern __shared__ int hist[];
+  int* mine = hist + kClusterWarps * vocab;
+  int* start = mine + vocab;
+  int* scratch = start + vocab;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
+  const int w0 = (rank * kClusterWarps + warp) * span, w1 = min(n, w0 + span);
+  int v[kClusterHeld];
+#pragma unroll
+  for (int j = 0; j < kClusterHeld; ++j) {
+    const int i = w0 + j * 32 + lane;
+    v[j] = i < w1 ? token_index(tok[i], vocab) : -1;
+  }
+  for (int i = threadIdx.x; i < kClusterWarps * vocab; i += kClusterThreads) hist[i] = 0;
+  __syncthreads();
+  int* next = hist + warp * vocab;
+#pragma unroll
+  for (int j = 0; j < kClusterHeld; ++j)
+    if (v[j] >= 0) atomicAdd(next + v[j], 1);
+  __syncthreads();
+  const int k = threadIdx.x;  // this thread's token
+  if (k < vocab) {
+    int sum = 0;
+#pragma unroll 8
+    for (int w = 0; w < kClusterWarps; ++w) {
+      const int c = hist[w * vocab + k];
+      hist[w * vocab + k] = sum;
+      sum += c;
+    }
+    mine[k] = sum;
+  }
+  cluster_sync_all();
+  int before = 0, count = 0, all;  // of the blocks before this one, and of all
+  if (k < vocab)
+#pragma unroll
+    for (int r = 0; r < kClusterBlocks; ++r) {
+      int c;
+      asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(cluster_addr(mine + k, r)) : "memory");
+      if (r < rank) before += c;
+      count += c;
+    }
+  cluster_sync_all();  // no block leaves while its totals are read
+  const int n_pieces = k < vocab ? pieces_of(count, rows) : 0;
+  const int base = block_prefix<kClusterThreads>(count, scratch, all);
+  const int first = block_prefix<kClusterThreads>(n_pieces, scratch, all);
+  if (k < vocab) {
+    start[k] = base + before;
+    if (k % kClusterBlocks == rank) {
+      const int size = rows_of_piece(count, rows);
+      for (int j = 0; j < n_pieces; ++j)
+        pieces[1 + first + j] = {k | n_pieces << 16, base + j * size, max(0, min(size, count - j * size)), first};
+      done[k] = 0;
+    }
+  }
+  if (rank == 0 && k == 0) pieces[0].at = all;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kClusterHeld; ++j) {
+    const unsigned same = __match_any_sync(~0u, v[j]);
+    const int place = __popc(same & ((1u << lane) - 1));
+    const int to = v[j] >= 0 ? next[v[j]] : 0;
+    __syncwarp();
+    if (v[j] >= 0) {
+      if (place == 0) next[v[j]] = to + __popc(same);
+      order[start[v[j]] + to + place] = w0 + j * 32 + lane;
+    }
+    __syncwarp();
+  }
+}
+
 // out (+)= scale * sum of N columns
 template <typename TD, int N>
 __device__ __forceinline__ void store_grad(TD* out, const float (&sum)[N], float scale, int accumulate) {
@@ -522,6 +606,29 @@ __global__ void __launch_bounds__(256) embed_zero_kernel(TD* dtable, long long l
   for (int c = threadIdx.x; c < d; c += 256) dtable[blockIdx.x * ld + c] = from_f32<TD>(0.f);
 }
 
+template <typename Tok>
+static cudaError_t launch_sort(const Tok* tok, int n, int vocab, int rows, Piece* pieces, int* done, int* order,
+                               cudaStream_t st) {
+  const auto kernel = embed_sort_kernel<Tok>;
+  const int warps = kClusterBlocks * kClusterWarps, span = ((n + warps - 1) / warps + 31) / 32 * 32;
+  const int smem = ((kClusterWarps + 2) * vocab + kClusterWarps) * 4;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(kClusterBlocks);
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = kClusterBlocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, tok, n, span, vocab, rows, pieces, done, order);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
 template <typename Tok, typename TG, typename TD, int N>
 static cudaError_t grad_run(const Tok* tok, long long n, const TG* dout, long long ld, int vocab, int d, float scale,
                             bool accumulate, TD* dtable, long long ld_dtable, int* w, cudaStream_t st) {
@@ -533,14 +640,19 @@ static cudaError_t grad_run(const Tok* tok, long long n, const TG* dout, long lo
     return cudaGetLastError();
   }
   const GradPlan p = grad_plan(n, vocab, d);
-  const size_t hist_bytes = (size_t)kSortWarps * vocab * 4;
-  embed_count_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes, st>>>(tok, n, vocab, p.tile, p.tiles, w + p.counts);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  embed_prefix_kernel<<<vocab, kPrefixThreads, 0, st>>>(w + p.counts, p.tiles, w + p.total, w + p.done);
   Piece* pieces = reinterpret_cast<Piece*>(w + p.pieces);
-  embed_order_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes + (2 * (vocab + 1) + kSortWarps) * 4, st>>>(
-      tok, n, vocab, p.tile, p.tiles, p.rows, w + p.counts, w + p.total, pieces, w + p.order);
+  cudaError_t e;
+  if (n <= kClusterRows) {
+    e = launch_sort(tok, (int)n, vocab, p.rows, pieces, w + p.done, w + p.order, st);
+  } else {
+    const size_t hist_bytes = (size_t)kSortWarps * vocab * 4;
+    embed_count_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes, st>>>(tok, n, vocab, p.tile, p.tiles, w + p.counts);
+    embed_prefix_kernel<<<vocab, kPrefixThreads, 0, st>>>(w + p.counts, p.tiles, w + p.total, w + p.done);
+    embed_order_kernel<Tok><<<p.tiles, kSortThreads, hist_bytes + (2 * (vocab + 1) + kSortWarps) * 4, st>>>(
+        tok, n, vocab, p.tile, p.tiles, p.rows, w + p.counts, w + p.total, pieces, w + p.order);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) return e;
   embed_sum_kernel<TG, TD, N><<<(unsigned)p.most, kSumThreads, 0, st>>>(
       dout, ld, d, q < kSumThreads ? q : kSumThreads, pieces, w + p.order, w + p.done,
       reinterpret_cast<float*>(w + p.part), scale, accumulate ? 1 : 0, dtable, ld_dtable);

@@ -148,7 +148,8 @@ def test_embed_backward(tr, dout_t, dtable_t, n, d, vocab, tok, skew):
     (40000, 12, 3, "bfloat16", True),        # more pieces than are kept of one token
     (300000, 7, 3, "float32", True),         # pieces longer than a block lists at once
     (300000, 300, 2, "float16", True),       # and columns in two rounds
-    (5000, 2052, 256, "float32", False), (4096, 300, 1024, "bfloat16", True), (4097, 8, 1024, "float16", False)])
+    (5000, 2052, 256, "float32", False), (49152, 20, 1024, "float32", True), (49153, 20, 1024, "float32", False),
+    (4096, 300, 1024, "bfloat16", True), (4097, 8, 1024, "float16", False)])
 def test_embed_backward_pieces(tr, n, d, vocab, dout_t, skew):
     """Long pieces, many pieces and wide rows; the sums in 64 bits by torch."""
     import torch
