@@ -325,14 +325,10 @@ __device__ __forceinline__ void leave(const Walk<V, G>& K, const Place& p, int p
 // and a store.
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
-  if constexpr (BYTES == 16) {
+  if constexpr (BYTES == 16)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-  } else if constexpr (BYTES >= 4) {
+  else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
-  } else {
-    const unsigned short x = __ldg(static_cast<const unsigned short*>(from));
-    asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(x) : "memory");
-  }
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -399,7 +395,14 @@ struct Carrier {
   template <int P>
   __device__ __forceinline__ void copy(Pack<T_, V>* stage, const T_* x, uint32_t row, int t, bool whole) const {
     const uint32_t to = smem_u32(stage) + at;
-    if (whole) {
+    if constexpr (kBytes == 2) {  // all loads, then all stores
+      unsigned short v[P];
+#pragma unroll
+      for (int k = 0; k < P; ++k)
+        v[k] = whole || t + k < len ? __ldg(reinterpret_cast<const unsigned short*>(row_at(x, row, k))) : 0;
+#pragma unroll
+      for (int k = 0; k < P; ++k) asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + k * kRow), "h"(v[k]) : "memory");
+    } else if (whole) {
 #pragma unroll
       for (int k = 0; k < P / kEvery; ++k) copy_async<kBytes>(to + k * kEvery * kRow, row_at(x, row, k * kEvery));
     } else {
@@ -832,7 +835,7 @@ cudaError_t launch_mingru_scan(const void* zh, int type, RowStrides zs, int B, i
       Shape s, n;
       cudaError_t e = shape_of<kernel, V, 32>(chains, T, P, scan_smem<E, V, 32>, s);
       if (e != cudaSuccess) return e;
-      if constexpr (Q && !(V == 2 && sizeof(E) == 4)) {  // those have groups enough
+      if constexpr (!(V == 2 && sizeof(E) == 4)) {  // those have groups enough
         constexpr auto narrow = mingru_scan_kernel<E, V, 16, Q>;
         if (s.reach < 148) {
           e = shape_of<narrow, V, 16>(chains, T, P, scan_smem<E, V, 16>, n);
@@ -876,14 +879,12 @@ cudaError_t launch_mingru_scan_grad(const void* zh, int type, RowStrides zs, int
       Shape s, n;
       cudaError_t e = shape_of<kernel, V, 32>(chains, T, kGradSteps, grad_smem<E, V, 32>, s);
       if (e != cudaSuccess) return e;
-      if constexpr (Q) {
+      if (s.reach < 148) {
         constexpr auto narrow = mingru_grad_kernel<E, V, 16, Q>;
-        if (s.reach < 148) {
-          e = shape_of<narrow, V, 16>(chains, T, kGradSteps, grad_smem<E, V, 16>, n);
-          if (e != cudaSuccess) return e;
-          if (half_reaches_further(n, s))
-            return launch_walk<narrow>(n, st, x, zs, T, d, by_d, chains, lengths, states, u, dhs, dh_last, o, dzs, dh0);
-        }
+        e = shape_of<narrow, V, 16>(chains, T, kGradSteps, grad_smem<E, V, 16>, n);
+        if (e != cudaSuccess) return e;
+        if (half_reaches_further(n, s))
+          return launch_walk<narrow>(n, st, x, zs, T, d, by_d, chains, lengths, states, u, dhs, dh_last, o, dzs, dh0);
       }
       return launch_walk<kernel>(s, st, x, zs, T, d, by_d, chains, lengths, states, u, dhs, dh_last, o, dzs, dh0);
     };
