@@ -5,6 +5,8 @@
 // captured into a CUDA graph.
 #include <cmath>
 
+#include "train_ops.cuh"
+
 namespace {
 
 // Checks shared by the entry points.  The message goes to a buffer of the
