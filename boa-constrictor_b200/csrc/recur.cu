@@ -198,11 +198,14 @@ struct Walk {
       mbar_init(full + 1, 1);
       fence_mbar_init();
     }
+    __syncwarp();  // the barrier is for whole warps
     cluster_sync_all();
   }
   // No block leaves before the others' last pushes have gone out.
   __device__ __forceinline__ void finish() const {
-    if (ranks > 1) cluster_sync_all();
+    if (ranks == 1) return;
+    __syncwarp();
+    cluster_sync_all();
   }
 };
 
@@ -512,11 +515,13 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     t += step;
     o += o_step;
   }
-  // the state after the last position: the walk's last team has applied all
+  // The state after the last position: the walk's last team has applied all.
+  // h_last may be h0: a push orders nothing before it, so only the cluster's
+  // last barrier says that the other blocks have read h0.
+  K.finish();
   if (h_last && at.in && at.rank == ranks - 1 && at.team == teams - 1)
 #pragma unroll
     for (int v = 0; v < V; ++v) h_last[at.chain + v] = s.v[v];
-  K.finish();
 }
 
 // ----------------------------------------------------------------- backward
@@ -647,10 +652,10 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     t -= step;
     o -= o_step;
   }
+  K.finish();  // dh0 may be dh_last, as above
   if (dh0 && at.in && at.rank == 0 && at.team == 0)
 #pragma unroll
     for (int v = 0; v < V; ++v) dh0[at.chain + v] = g.v[v];
-  K.finish();
 }
 
 // ------------------------------------------------------------- few positions

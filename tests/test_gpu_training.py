@@ -351,6 +351,33 @@ def test_mingru_state_in_place_over_steps(tr, T):
     _close(state, *ref["last"], "float32")
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("B,T,d", [(1, 700, 64), (1, 2000, 160), (2, 2049, 32), (3, 900, 33), (300, 40, 64)])
+def test_mingru_states_in_place_both_ways(tr, dtype, B, T, d):
+    """The state and its gradient updated in their own buffers give the bits
+    of separate ones, with one block a group of chains and with several (which
+    all read the buffer that one of them writes)."""
+    import torch
+    L = tr.lib()
+    torch.manual_seed(T + d)
+    r = lambda *s: torch.randn(*s, device="cuda")
+    zh, dh = r(B, T, 2 * d).to(getattr(torch, dtype)), r(B, T, d).to(getattr(torch, dtype))
+    h0, dl = r(B, d), r(B, d)
+    h, last, saved = tr.mingru_scan(zh, h0, save_states=True)
+    dzh, dh0 = tr.mingru_scan_backward(zh, saved, dh, dl)
+    kind = {"float32": 0, "float16": 1, "bfloat16": 2}[dtype]
+    stream = torch.cuda.current_stream().cuda_stream
+    for _ in range(20):
+        s = h0.clone()
+        h2, _ = tr.mingru_scan(zh, s, h_last=s)
+        assert torch.equal(s, last) and torch.equal(h2, h)
+        g, dzh2 = dl.clone(), torch.empty_like(dzh)
+        assert L.boa_mingru_scan_backward(zh.data_ptr(), kind, 2 * d, T * 2 * d, B, T, d, None, saved.data_ptr(),
+                                          dh.data_ptr(), d, T * d, g.data_ptr(), dzh2.data_ptr(), 2 * d, T * 2 * d,
+                                          g.data_ptr(), stream) == 0
+        assert torch.equal(g, dh0) and torch.equal(dzh2, dzh)
+
+
 def test_mingru_takes_an_expanded_gradient(tr):
     import torch
     zh, h0, _, _, _ = _case(torch, np.random.default_rng(9), 4, 150, 32, "float32")
