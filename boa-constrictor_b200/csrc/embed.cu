@@ -398,6 +398,7 @@ embed_sort_kernel(const Tok* __restrict__ tok, int n, int span, int vocab, int r
     }
     mine[k] = sum;
   }
+  __syncwarp();  // the barrier is for whole warps, and the alphabet may end inside one
   cluster_sync_all();
   int before = 0, count = 0, all;  // of the blocks before this one, and of all
   if (k < vocab)
@@ -408,6 +409,7 @@ embed_sort_kernel(const Tok* __restrict__ tok, int n, int span, int vocab, int r
       if (r < rank) before += c;
       count += c;
     }
+  __syncwarp();
   cluster_sync_all();  // no block leaves while its totals are read
   const int n_pieces = k < vocab ? pieces_of(count, rows) : 0;
   const int base = block_prefix<kClusterThreads>(count, scratch, all);
