@@ -362,6 +362,7 @@ embed_order_kernel(const Tok* __restrict__ tok, long long n, int vocab, int tile
 constexpr int kClusterBlocks = 8, kClusterThreads = 1024, kClusterWarps = kClusterThreads / 32;
 constexpr int kClusterHeld = 6;   // tokens of a lane
 constexpr int kClusterRows = kClusterBlocks * kClusterThreads * kClusterHeld;
+constexpr int cluster_smem(int vocab) { return ((kClusterWarps + 2) * vocab + kClusterWarps) * 4; }
 
 template <typename Tok>
 __global__ void __launch_bounds__(kClusterThreads)
@@ -614,13 +615,13 @@ static cudaError_t launch_sort(const Tok* tok, int n, int vocab, int rows, Piece
                                cudaStream_t st) {
   const auto kernel = embed_sort_kernel<Tok>;
   const int warps = kClusterBlocks * kClusterWarps, span = ((n + warps - 1) / warps + 31) / 32 * 32;
-  const int smem = ((kClusterWarps + 2) * vocab + kClusterWarps) * 4;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  // the limit is the kernel's, whatever thread launches it: always the largest alphabet's
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, cluster_smem(kMaxVocab));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(kClusterBlocks);
   cfg.blockDim = dim3(kClusterThreads);
-  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.dynamicSmemBytes = (size_t)cluster_smem(vocab);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;

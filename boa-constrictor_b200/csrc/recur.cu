@@ -760,10 +760,11 @@ static cudaError_t shape_of(long long chains, int T, int P, M smem, Shape& s) {
   s.threads = s.teams * s.per * G;
   if (s.threads < 32) s.threads = 32;  // two half-warp teams, of two groups
   if (s.threads > s.teams * s.per * G) s.per = s.threads / (s.teams * G);
-  const size_t most_smem = smem(s.threads, kMaxCluster);
   // clusters are packed: two of their blocks on one SM while another stays
   // empty, unless a block takes more than half of the shared memory
-  const size_t alone = most_smem < 116 * 1024 ? 116 * 1024 : most_smem;
+  const size_t widest = smem(alone_warps<V>() * 32, kMaxCluster), alone = widest < 116 * 1024 ? 116 * 1024 : widest;
+  // The limit belongs to the kernel on the device, not to this launch: a
+  // constant, so that two threads that launch different shapes agree on it.
   const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)alone);
   if (e != cudaSuccess) return e;
   if (s.teams == block_teams && groups * 2 <= 148)

@@ -1,0 +1,124 @@
+"""How the training operators (boa_b200.training) are called: from several
+threads at once, in one captured graph, after a call that failed."""
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+KIND = {"float32": 0, "float16": 1, "bfloat16": 2}
+
+
+@pytest.fixture(scope="module")
+def tr(boa):
+    from boa_b200 import training
+    return training
+
+
+def _scan_call(tr, torch, B, T, d, dtype, back, seed=0):
+    """-> (call(stream) -> status, the tensors that it writes)"""
+    L, g = tr.lib(), torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    zh, dh = r(B, T, 2 * d).to(getattr(torch, dtype)), r(B, T, d).to(getattr(torch, dtype))
+    h, saved = torch.empty_like(dh), torch.empty(L.boa_mingru_states_floats(B, T, d), device="cuda")
+    last, dzh, dh0 = r(B, d), torch.empty_like(zh), r(B, d)
+    k, w = KIND[dtype], 2 * d
+
+    def forward(st):
+        return L.boa_mingru_scan(zh.data_ptr(), k, w, T * w, B, T, d, None, None, h.data_ptr(), d, T * d,
+                                 last.data_ptr(), saved.data_ptr(), st)
+
+    def backward(st):
+        return L.boa_mingru_scan_backward(zh.data_ptr(), k, w, T * w, B, T, d, None, saved.data_ptr(), dh.data_ptr(),
+                                          d, T * d, None, dzh.data_ptr(), w, T * w, dh0.data_ptr(), st)
+    assert forward(torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    return (backward, [dzh, dh0]) if back else (forward, [h, last, saved])
+
+
+def _grad_call(tr, torch, n, vocab, d, seed=0):
+    L, g = tr.lib(), torch.Generator(device="cuda").manual_seed(seed)
+    tok = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    dout = torch.randn(n, d, generator=g, device="cuda")
+    out = torch.empty(vocab, d, device="cuda")
+    ws = torch.empty(L.boa_embed_backward_workspace(n, vocab, d), dtype=torch.uint8, device="cuda")
+
+    def call(st):
+        return L.boa_embed_backward(tok.data_ptr(), 1, n, dout.data_ptr(), 0, d, vocab, d, 1.0, 0, out.data_ptr(), 0, d,
+                                    ws.data_ptr(), ws.numel(), st)
+    return call, [out]
+
+
+# two shapes of one kernel that need different amounts of shared memory
+PAIRS = {
+    "scan_f32": lambda tr, t: (_scan_call(tr, t, 8, 700, 256, "float32", False), _scan_call(tr, t, 75, 64, 64, "float32", False)),
+    "scan_bf16": lambda tr, t: (_scan_call(tr, t, 16, 700, 256, "bfloat16", False), _scan_call(tr, t, 150, 64, 64, "bfloat16", False)),
+    "back_f32": lambda tr, t: (_scan_call(tr, t, 8, 700, 256, "float32", True), _scan_call(tr, t, 75, 64, 64, "float32", True)),
+    "back_bf16": lambda tr, t: (_scan_call(tr, t, 16, 700, 256, "bfloat16", True), _scan_call(tr, t, 150, 64, 64, "bfloat16", True)),
+    "narrow_f32": lambda tr, t: (_scan_call(tr, t, 1, 3000, 64, "float32", False), _scan_call(tr, t, 1, 20, 64, "float32", False)),
+    "table": lambda tr, t: (_grad_call(tr, t, 5000, 1024, 8), _grad_call(tr, t, 5000, 16, 8)),
+}
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+def test_two_threads_launch_different_shapes(tr, boa, pair):
+    """Calls of one kernel with much and with little shared memory, from two
+    threads at once: neither fails, and both give what they give alone."""
+    import torch
+    calls = PAIRS[pair](tr, torch)
+    main = torch.cuda.current_stream().cuda_stream
+    want = []
+    for call, outs in calls:
+        assert call(main) == 0
+        torch.cuda.synchronize()
+        want.append([x.clone() for x in outs])
+    streams, failed = [torch.cuda.Stream() for _ in calls], []
+    torch.cuda.synchronize()
+    ready = threading.Barrier(len(calls))
+
+    def work(k):
+        torch.cuda.set_device(0)
+        call, st = calls[k][0], streams[k].cuda_stream
+        ready.wait()
+        for i in range(3000):
+            rc = call(st)
+            if rc != 0:
+                failed.append((k, i, rc, tr.lib().boa_last_error(None)))
+                break
+            if i % 256 == 255:
+                streams[k].synchronize()
+    ts = [threading.Thread(target=work, args=(k,)) for k in range(len(calls))]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for (_, outs), ref in zip(calls, want):
+        for x, y in zip(outs, ref):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("pair", PAIRS)
+def test_different_shapes_in_one_graph(tr, pair):
+    """A graph that holds a launch with much shared memory, then one with
+    little, is instantiated after both."""
+    import torch
+    calls = PAIRS[pair](tr, torch)
+    s = torch.cuda.Stream()
+    for call, _ in calls:
+        assert call(s.cuda_stream) == 0
+    s.synchronize()
+    want = [[x.clone() for x in outs] for _, outs in calls]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        for call, _ in calls:
+            assert call(s.cuda_stream) == 0
+    for _, outs in calls:
+        [x.zero_() for x in outs]
+    g.replay()
+    torch.cuda.synchronize()
+    for (_, outs), ref in zip(calls, want):
+        for x, y in zip(outs, ref):
+            assert torch.equal(x, y)
