@@ -19,6 +19,7 @@
 // gradient 191 us; profiled one by one, the row sums take 169 us (6.4 TB/s) and
 // the sort's three launches 28 us.
 #include "kernels.cuh"
+#include "pieces.h"
 #include "ptx.cuh"
 #include "train_ops.cuh"
 
@@ -131,7 +132,6 @@ constexpr int kTile = kSortThreads * kSortHeld;            // least tokens of a 
 constexpr int kMaxTiles = 1024;
 constexpr int kSumThreads = 256;
 constexpr int kSumChunk = 1024;    // positions of a piece in shared memory at once
-constexpr int kMaxPieces = 256;    // of one token: what its last block adds up
 constexpr int kSmallRows = 4096;   // up to here one kernel does all
 constexpr int kSmallPacks = 16;
 
@@ -163,14 +163,6 @@ static GradPlan grad_plan(long long n, int vocab, int d) {
 }
 size_t embed_grad_workspace(long long n, int vocab, int d) {
   return n > kSmallRows ? grad_plan(n, vocab, d).words * 4 : 0;
-}
-// Rows of a token's pieces, and their number (one, of no rows, for a token that does not occur).
-__device__ __forceinline__ int rows_of_piece(int total, int rows) {
-  return max(rows, (total + kMaxPieces - 1) / kMaxPieces);
-}
-__device__ __forceinline__ int pieces_of(int total, int rows) {
-  const int r = rows_of_piece(total, rows);
-  return max(1, (total + r - 1) / r);
 }
 struct alignas(16) Piece {
   int tok_pieces;  // token, and its pieces << 16
