@@ -43,8 +43,6 @@ token_loss_kernel(const T_* logits, long long ld, long long rows, int vocab, con
     return;
   }
   const T_* x = logits + row * ld;
-  // the target's logit, read by all lanes before the reductions that every
-  // lane of the row passes, and so before any gradient is written over it
   const float hit = to_f32(x[target]);
   float v[C][N];
   float m = -INFINITY;
@@ -79,6 +77,7 @@ token_loss_kernel(const T_* logits, long long ld, long long rows, int vocab, con
   for (int o = L / 2; o; o >>= 1) sum += __shfl_xor_sync(lanes, sum, o);
   if (loss && lane == 0) loss[row] = sum == 0.f ? INFINITY : logf(sum) - (hit - m) * inv_t;
   if (grad) {
+    __syncwarp(lanes);  // in place: all logits, the target's too, are read before a gradient is written over them
     const float w = sum == 0.f ? 0.f : (dloss ? dloss[row] * grad_scale : grad_scale) * inv_t;
     const float r = sum == 0.f ? 0.f : w / sum;
     const int pack = target / N, own = pack % L == lane ? pack / L : -1;  // the pack that holds the target
