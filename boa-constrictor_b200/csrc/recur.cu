@@ -125,6 +125,10 @@ __device__ __forceinline__ float max_or_nan(float x, float y) {
 // below 2^-126, which the instruction flushes: from there down z is 0 and
 // a is 1, exactly (the candidate then has no weight).  A closed gate so keeps
 // the state however many positions long.
+//
+// For zl >= 0 a is taken as e z: 1 - z would leave few of its digits, and none
+// from zl = 17 on, and the gate's gradient is proportional to it.  Below 0
+// the difference has all digits, and e z would not be 1 for a closed gate.
 template <int V>
 struct Cell {
   Vec<V> a, b;  // 1 - z, z c
@@ -142,7 +146,7 @@ __device__ __forceinline__ Cell<V> mingru_cell(const Vec<V>& zl, const Vec<V>& h
     // hr + 1/2 lies below sigmoid(hr) for hr < 0 (slopes 1 and at most 1/4
     // from the same value at 0), and above sigmoid(-hr) <= 1/2 otherwise
     const float c = fmaxf(hr.v[v] + 0.5f, low);
-    k.a.v[v] = 1.f - z;
+    k.a.v[v] = e <= 1.f ? e * z : 1.f - z;
     k.b.v[v] = z * c;
     k.z.v[v] = z;
     if (GRAD) k.w.v[v] = z * (hr.v[v] >= 0.f ? 1.f : __fmaf_rn(-low, low, low));
