@@ -16,11 +16,17 @@ int train_fail(int code, const char* fn, const char* what) {
   std::snprintf(t_call_error, sizeof t_call_error, "%s: %s", fn, what);
   return code;
 }
-// A launch into a stream that is not of the current device fails as an
-// invalid handle.  Asking for the stream's device beforehand is no choice:
-// the query ends a stream capture.
-int train_launch(const char* fn, cudaError_t e) {
+// Runs a launcher.  An error that an earlier call left behind is not this
+// call's, and this call's is not left to a later one: a launch's outcome is
+// read back from the thread's last error.  A launch into a stream that is not
+// of the current device fails as an invalid handle.  Asking for the stream's
+// device beforehand is no choice: the query ends a stream capture.
+template <typename F>
+int train_launch(const char* fn, F&& launch) {
+  cudaGetLastError();
+  const cudaError_t e = launch();
   if (e == cudaSuccess) return BOA_OK;
+  cudaGetLastError();
   if (e == cudaErrorInvalidResourceHandle)
     return train_fail(BOA_E_INVALID, fn, "the stream belongs to another device");
   return train_fail(BOA_E_CUDA, fn, cudaGetErrorString(e));
@@ -65,8 +71,10 @@ int boa_embed(const void* d_tokens, int token_type, int64_t n, const void* d_tab
   BOA_REQUIRE(token_aligned(d_tokens, token_type) && elem_aligned(d_table, table_type) &&
                   elem_aligned(d_out, out_type),
               "a buffer is not aligned to its element");
-  return train_launch(__func__, boa::launch_embed(d_tokens, token_type, n, d_table, table_type, ld_table, vocab, d,
-                                                  scale, d_out, out_type, ld_out, (cudaStream_t)stream));
+  return train_launch(__func__, [&] {
+    return boa::launch_embed(d_tokens, token_type, n, d_table, table_type, ld_table, vocab, d, scale, d_out, out_type,
+                             ld_out, (cudaStream_t)stream);
+  });
 }
 
 size_t boa_embed_backward_workspace(int64_t n, int vocab, int d) {
@@ -92,10 +100,10 @@ int boa_embed_backward(const void* d_tokens, int token_type, int64_t n, const vo
     BOA_REQUIRE(need == 0 || (d_workspace && boa::aligned_to(d_workspace, 16) && workspace_bytes >= need),
                 "the workspace is null, not aligned to 16 bytes or below boa_embed_backward_workspace");
   }
-  return train_launch(__func__,
-                      boa::launch_embed_grad(d_tokens, token_type, n, d_dout, dout_type, ld_dout, vocab, d, scale,
-                                             accumulate != 0, d_dtable, dtable_type, ld_dtable, d_workspace,
-                                             (cudaStream_t)stream));
+  return train_launch(__func__, [&] {
+    return boa::launch_embed_grad(d_tokens, token_type, n, d_dout, dout_type, ld_dout, vocab, d, scale, accumulate != 0,
+                                  d_dtable, dtable_type, ld_dtable, d_workspace, (cudaStream_t)stream);
+  });
 }
 
 uint64_t boa_mingru_states_floats(int n_chunks, int T, int d) {
@@ -117,9 +125,10 @@ int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk
   BOA_REQUIRE(elem_aligned(d_zh, type) && elem_aligned(d_h, type) && boa::aligned_to(d_lengths, 4) &&
                   boa::aligned_to(d_h0, 4) && boa::aligned_to(d_h_last, 4) && boa::aligned_to(d_states, 4),
               "a buffer is not aligned to its element");
-  return train_launch(__func__, boa::launch_mingru_scan(d_zh, type, {zh_row, zh_chunk}, n_chunks, T, d, d_lengths,
-                                                        d_h0, d_h, {h_row, h_chunk}, d_h_last, d_states,
-                                                        (cudaStream_t)stream));
+  return train_launch(__func__, [&] {
+    return boa::launch_mingru_scan(d_zh, type, {zh_row, zh_chunk}, n_chunks, T, d, d_lengths, d_h0, d_h, {h_row,
+                                   h_chunk}, d_h_last, d_states, (cudaStream_t)stream);
+  });
 }
 
 int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
@@ -140,9 +149,11 @@ int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t
                   boa::aligned_to(d_lengths, 4) && boa::aligned_to(d_states, 4) && boa::aligned_to(d_dh_last, 4) &&
                   boa::aligned_to(d_dh0, 4),
               "a buffer is not aligned to its element");
-  return train_launch(__func__, boa::launch_mingru_scan_grad(d_zh, type, {zh_row, zh_chunk}, n_chunks, T, d,
-                                                             d_lengths, d_states, d_dh, {dh_row, dh_chunk}, d_dh_last,
-                                                             d_dzh, {dzh_row, dzh_chunk}, d_dh0, (cudaStream_t)stream));
+  return train_launch(__func__, [&] {
+    return boa::launch_mingru_scan_grad(d_zh, type, {zh_row, zh_chunk}, n_chunks, T, d, d_lengths, d_states, d_dh,
+                                        {dh_row, dh_chunk}, d_dh_last, d_dzh, {dzh_row, dzh_chunk}, d_dh0,
+                                        (cudaStream_t)stream);
+  });
 }
 
 int boa_token_loss(const void* d_logits, int type, int64_t ld, int64_t n_rows, int vocab, const void* d_targets,
@@ -161,9 +172,10 @@ int boa_token_loss(const void* d_logits, int type, int64_t ld, int64_t n_rows, i
   BOA_REQUIRE(elem_aligned(d_logits, type) && token_aligned(d_targets, token_type) && boa::aligned_to(d_dloss, 4) &&
                   boa::aligned_to(d_loss, 4) && elem_aligned(d_dlogits, type),
               "a buffer is not aligned to its element");
-  return train_launch(__func__, boa::launch_token_loss(d_logits, type, ld, n_rows, vocab, d_targets, token_type,
-                                                       inv_temperature, d_dloss, grad_scale, d_loss, d_dlogits,
-                                                       ld_dlogits, (cudaStream_t)stream));
+  return train_launch(__func__, [&] {
+    return boa::launch_token_loss(d_logits, type, ld, n_rows, vocab, d_targets, token_type, inv_temperature, d_dloss,
+                                  grad_scale, d_loss, d_dlogits, ld_dlogits, (cudaStream_t)stream);
+  });
 }
 
 }  // extern "C"

@@ -122,3 +122,59 @@ def test_different_shapes_in_one_graph(tr, pair):
     for (_, outs), ref in zip(calls, want):
         for x, y in zip(outs, ref):
             assert torch.equal(x, y)
+
+
+class _Driver:
+    """The few driver calls that a stream capture needs, on a stream of its own."""
+
+    def __init__(self):
+        self.cu = C.CDLL("libcuda.so.1")
+        self.stream = C.c_void_p()
+        assert self.cu.cuStreamCreate(C.byref(self.stream), 0) == 0  # waits on the legacy stream, and it on this one
+
+    def begin(self):
+        assert self.cu.cuStreamBeginCapture_v2(self.stream, 0) == 0
+
+    def end(self):
+        graph = C.c_void_p()
+        rc = self.cu.cuStreamEndCapture(self.stream, C.byref(graph))
+        if graph.value:
+            self.cu.cuGraphDestroy(graph)
+        return rc
+
+
+@pytest.mark.parametrize("failing", ["scan", "back", "table", "small_table", "step"])
+@pytest.mark.parametrize("then", ["scan", "table", "step"])
+def test_a_failed_launch_is_not_a_later_calls_error(tr, boa, failing, then):
+    """A launch into the legacy stream while another stream that waits on it is
+    captured is refused by the driver; the next call is sound again."""
+    import torch
+    make = {"scan": lambda: _scan_call(tr, torch, 2, 100, 32, "float32", False),
+            "back": lambda: _scan_call(tr, torch, 2, 100, 32, "float32", True),
+            "step": lambda: _scan_call(tr, torch, 2, 1, 32, "float32", False),
+            "table": lambda: _grad_call(tr, torch, 5000, 64, 8), "small_table": lambda: _grad_call(tr, torch, 50, 64, 8)}
+    bad, (good, outs) = make[failing]()[0], make[then]()
+    main = torch.cuda.current_stream().cuda_stream
+    assert good(main) == 0
+    torch.cuda.synchronize()
+    want = [x.clone() for x in outs]
+    torch.cuda.synchronize()
+    drv = _Driver()
+    drv.begin()
+    rc = bad(None)
+    ended = drv.end()
+    assert rc == boa.BOA_E_CUDA and ended != 0, (rc, ended)
+    assert b"captur" in tr.lib().boa_last_error(None)
+    for _ in range(2):
+        assert good(main) == 0, tr.lib().boa_last_error(None)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+def test_an_earlier_failure_elsewhere_is_not_this_calls_error(tr, boa):
+    import torch
+    call, _ = _scan_call(tr, torch, 2, 1, 32, "float32", False)
+    with pytest.raises(boa.BoaError):
+        boa.Model("/nonexistent.bin", "mingru", 64, 2, device=99)
+    assert call(torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
