@@ -124,6 +124,7 @@ SIGNATURES = {
                                   _vp, _vp, _vp]),
     "boa_mingru_scan_backward": (C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _i64,
                                            _i64, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "boa_selftest_walk_timeout": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_uint32, _f32p]),
     "boa_token_loss": (C.c_int, [_vp, C.c_int, _i64, _i64, C.c_int, _vp, C.c_int, C.c_float, _vp, C.c_float, _vp,
                                  _vp, _i64, _vp]),
     "boa_pyrc_decode_step": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),

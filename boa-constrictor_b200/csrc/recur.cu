@@ -182,7 +182,9 @@ struct Walk {
   uint64_t* full;   // [2]: barriers that count the bytes pushed into `block` (ranks > 1)
   uint8_t* stages;
   int teams, ranks;
-  __device__ __forceinline__ Walk(uint8_t* at, int ranks_, bool both) : teams(blockDim.x / G), ranks(ranks_) {
+  uint64_t limit_ns;  // of a wait
+  __device__ __forceinline__ Walk(uint8_t* at, int ranks_, bool both, uint64_t limit_ns_ = kWaitLimitNs)
+      : teams(blockDim.x / G), ranks(ranks_), limit_ns(limit_ns_) {
     maps = reinterpret_cast<Map<V>*>(at);
     forward = maps + 2 * G * teams;
     block = forward + (both ? 2 * G * teams : 0);
@@ -205,11 +207,15 @@ struct Walk {
     __syncwarp();  // the barrier is for whole warps
     cluster_sync_all();
   }
-  // No block leaves before the others' last pushes have gone out.
-  __device__ __forceinline__ void finish() const {
+  // No block leaves before the others' last pushes have gone out.  One that
+  // has stopped waiting did not see them arrive, and stays a little longer.
+  __device__ __forceinline__ void finish(bool waiting) const {
     if (ranks == 1) return;
     __syncwarp();
     cluster_sync_all();
+    if (!waiting)
+      for (const uint64_t t0 = global_ns(); global_ns() - t0 < 100000;) {
+      }
   }
 };
 
@@ -266,13 +272,16 @@ __device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) 
       : "memory");
   return ok != 0;
 }
-// Waits for a phase.  When the wait runs out `waiting` is cleared: the walk's
-// state becomes NaN, and the walk goes on without waiting again (a handle-free
-// call has no error word to set).
-__device__ __forceinline__ void await_maps(uint32_t bar, uint32_t parity, bool& waiting) {
+// Waits for a phase.  When the wait runs out `waiting` is cleared: this
+// thread's state becomes NaN, and with it all that it writes from there on (a
+// handle-free call has no error word to set).  It neither waits nor pushes
+// again: a slot that it filled without waiting could still be in use, and
+// would give another block a wrong map.  The others miss its maps and run
+// out in the next step, so every value written is right or NaN.
+__device__ __forceinline__ void await_maps(uint32_t bar, uint32_t parity, uint64_t limit_ns, bool& waiting) {
   if (waiting && !try_wait_cluster(bar, parity)) {
     const uint64_t t0 = global_ns();
-    while (waiting && !try_wait_cluster(bar, parity)) waiting = global_ns() - t0 <= kWaitLimitNs;
+    while (waiting && !try_wait_cluster(bar, parity)) waiting = global_ns() - t0 <= limit_ns;
   }
   __syncwarp();  // lanes may leave the loop apart
 }
@@ -298,16 +307,16 @@ __device__ __forceinline__ Vec<V> exchange(const Walk<V, G>& K, const Place& p, 
   if (p.ranks == 1) {
     s = step == 0 ? x : K.state[parity * G + p.lane];
   } else {
-    if (threadIdx.x == 0) mbar_arrive_expect_tx(K.full + parity, (uint32_t)(p.ranks * G * sizeof(Map<V>)));
+    if (threadIdx.x == 0 && waiting) mbar_arrive_expect_tx(K.full + parity, (uint32_t)(p.ranks * G * sizeof(Map<V>)));
     const int turn = REVERSE ? p.ranks - 1 - p.rank : p.rank;
-    if (p.team < p.ranks) {  // team r takes the block's map to block r
+    if (p.team < p.ranks && waiting) {  // team r takes the block's map to block r
       Map<V> all = maps[0];
 #pragma unroll 4
       for (int w = 1; w < p.teams; ++w) all = then<V>(all, maps[w * G]);
       push_map<V>(cluster_addr(K.block + (parity * p.ranks + turn) * G + p.lane, (uint32_t)p.team), all,
                   cluster_addr(K.full + parity, (uint32_t)p.team));
     }
-    await_maps(smem_u32(K.full + parity), (uint32_t)(step >> 1) & 1u, waiting);
+    await_maps(smem_u32(K.full + parity), (uint32_t)(step >> 1) & 1u, K.limit_ns, waiting);
     if (!waiting) x = all_of<V>(__int_as_float(0x7fffffff));
     for (int r = 0; r < p.ranks; ++r) {
       if (r == turn) s = x;
@@ -522,7 +531,7 @@ mingru_scan_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
   // The state after the last position: the walk's last team has applied all.
   // h_last may be h0: a push orders nothing before it, so only the cluster's
   // last barrier says that the other blocks have read h0.
-  K.finish();
+  K.finish(waiting);
   if (h_last && at.in && at.rank == ranks - 1 && at.team == teams - 1)
 #pragma unroll
     for (int v = 0; v < V; ++v) h_last[at.chain + v] = s.v[v];
@@ -656,10 +665,42 @@ mingru_grad_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastD
     t -= step;
     o -= o_step;
   }
-  K.finish();  // dh0 may be dh_last, as above
+  K.finish(waiting);  // dh0 may be dh_last, as above
   if (dh0 && at.in && at.rank == 0 && at.team == 0)
 #pragma unroll
     for (int v = 0; v < V; ++v) dh0[at.chain + v] = g.v[v];
+}
+
+// A walk of a cluster of two blocks whose second stops pushing its maps at step `silent`: what the exchange
+// gives each thread, [step][thread of the cluster].  Every run of positions adds 1.
+__global__ void __launch_bounds__(64)
+walk_selftest_kernel(int steps, int silent, FastDiv by_32, uint64_t limit_ns, float* out) {
+  extern __shared__ __align__(16) uint8_t walk_smem[];
+  const Walk<1, 32> K(walk_smem, 2, false, limit_ns);
+  K.start();
+  const Place at = place_of<1, 32>(2, 2, 32, 32, by_32);
+  Vec<1> walk = all_of<1>(0.f);
+  bool waiting = true;
+  for (int i = 0; i < steps; ++i) {
+    if (i >= silent && at.rank == 1) waiting = false;
+    out[(i * 2 + at.rank) * 64 + threadIdx.x] =
+        exchange<1, 32, false>(K, at, i, {all_of<1>(1.f), all_of<1>(1.f)}, walk, waiting).v[0];
+  }
+  K.finish(waiting);
+}
+cudaError_t launch_walk_selftest(int steps, int silent, uint64_t limit_ns, float* out, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(64);
+  cfg.dynamicSmemBytes = Walk<1, 32>::bytes(64, 2, false);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, walk_selftest_kernel, steps, silent, fast_div(32), limit_ns, out);
 }
 
 // ------------------------------------------------------------- few positions

@@ -2,7 +2,7 @@
 // stepped with: handle-free, on caller-owned device buffers and the caller's
 // stream, like the step-wise coder (coder_api.cu).  Arguments are checked
 // here; nothing is allocated and nothing is synchronised, so every call can be
-// captured into a CUDA graph.
+// captured into a CUDA graph (but for the walk's self-test).
 #include <cmath>
 
 #include "train_ops.cuh"
@@ -153,6 +153,29 @@ int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t
     return boa::launch_mingru_scan_grad(d_zh, type, {zh_row, zh_chunk}, n_chunks, T, d, d_lengths, d_states, d_dh,
                                         {dh_row, dh_chunk}, d_dh_last, d_dzh, {dzh_row, dzh_chunk}, d_dh0,
                                         (cudaStream_t)stream);
+  });
+}
+
+int boa_selftest_walk_timeout(int device, int n_steps, int silent_from, uint32_t limit_us, float* out) {
+  int n_dev = 0;
+  if (cudaGetDeviceCount(&n_dev) != cudaSuccess) {
+    cudaGetLastError();
+    n_dev = 0;
+  }
+  BOA_REQUIRE(device >= 0 && device < n_dev, "no such CUDA device");
+  BOA_REQUIRE(n_steps >= 1 && n_steps <= 64 && silent_from >= 0, "n_steps must be 1 .. 64, silent_from not negative");
+  BOA_REQUIRE(limit_us >= 1 && limit_us <= 1000000u, "limit_us must be in [1, 1e6]");
+  BOA_REQUIRE(out, "null buffer");
+  DeviceGuard dev(device);
+  return train_launch(__func__, [&] {
+    const size_t bytes = (size_t)n_steps * 128 * sizeof(float);
+    float* d_out = nullptr;
+    cudaError_t e = cudaMalloc(&d_out, bytes);
+    if (e != cudaSuccess) return e;
+    e = boa::launch_walk_selftest(n_steps, silent_from, limit_us * 1000ull, d_out, nullptr);
+    if (e == cudaSuccess) e = cudaMemcpy(out, d_out, bytes, cudaMemcpyDeviceToHost);
+    cudaFree(d_out);
+    return e;
   });
 }
 

@@ -169,6 +169,9 @@ cudaError_t launch_mingru_scan_grad(const void* zh, int type, RowStrides zs, int
                                     const float* states, const void* dh, RowStrides dhs, const float* dh_last,
                                     void* dzh, RowStrides dzs, float* dh0, cudaStream_t st);
 
+// What the walk's exchange gives when one of a cluster's two blocks falls silent: [steps][128], see recur.cu
+cudaError_t launch_walk_selftest(int steps, int silent, uint64_t limit_ns, float* out, cudaStream_t st);
+
 // Next-token cross entropy per row and its gradient; see loss.cu
 cudaError_t launch_token_loss(const void* logits, int type, long long ld, long long rows, int vocab,
                               const void* targets, int tok_t, float inv_t, const float* dloss, float grad_scale,

@@ -310,6 +310,21 @@ int boa_mingru_scan_backward(const void* d_zh, int type, int64_t zh_row, int64_t
                              int64_t dh_chunk, const float* d_dh_last, void* d_dzh, int64_t dzh_row,
                              int64_t dzh_chunk, float* d_dh0, void* stream);
 
+/* Long sequences of few chains are walked by several blocks that hand maps to
+ * each other.  Their waits are bounded like all of this library (2 s of wall
+ * time, which only a GPU that stops the kernel in the middle reaches), and
+ * these calls have no handle whose error word could be set: where a wait runs
+ * out the states, or gradients, from there on are NaN.  No other value is
+ * affected, the call still ends, and the context stays usable.
+ *
+ * Self-test of that: two blocks exchange the maps x -> x + 1 of their two
+ * teams for n_steps (1 .. 64) steps; the second block falls silent at step
+ * silent_from (n_steps or more: never).  Waits are cut to limit_us
+ * microseconds (1 .. 1e6).  out (host) [n_steps][2 blocks][2 teams][32 lanes]
+ * receives the states that enter each team's positions: 4 step + 2 block +
+ * team, and NaN once a wait has run out.  Synchronises. */
+int boa_selftest_walk_timeout(int device, int n_steps, int silent_from, uint32_t limit_us, float* out);
+
 /* Next-token cross entropy of n_rows rows of vocab <= 1024 logits, and its
  * gradient, in one pass:
  *   loss[i] = -ln p[target], p = softmax(inv_temperature * logits[i])

@@ -178,3 +178,24 @@ def test_an_earlier_failure_elsewhere_is_not_this_calls_error(tr, boa):
         boa.Model("/nonexistent.bin", "mingru", 64, 2, device=99)
     assert call(torch.cuda.current_stream().cuda_stream) == 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("silent", [0, 1, 2, 3, 5, 8])
+def test_a_wait_that_runs_out_gives_nan_and_nothing_else(tr, boa, silent):
+    """One of two blocks falls silent: from then on every state is NaN, before
+    it every state is right, the kernel ends soon and the context goes on."""
+    import time
+    import torch
+    call, outs = _scan_call(tr, torch, 1, 700, 64, "float32", False)  # by clusters
+    torch.cuda.synchronize()
+    want = [x.clone() for x in outs]
+    got = np.zeros((8, 2, 2, 32), np.float32)
+    t0 = time.monotonic()
+    rc = tr.lib().boa_selftest_walk_timeout(0, 8, silent, 20000, got.ctypes.data_as(C.POINTER(C.c_float)))
+    assert rc == 0 and time.monotonic() - t0 < 5
+    step, block, team, _ = np.indices(got.shape)
+    assert np.isnan(got[silent:]).all()
+    assert (got[:silent] == (4 * step + 2 * block + team)[:silent]).all()
+    assert call(torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(outs, want))
