@@ -12,10 +12,17 @@ token; ``mingru_scan`` / ``mingru_scan_backward`` run the minGRU recurrence
 over whole sequences (with one position, the decode step); ``token_loss``
 gives the next-token loss and its gradient in one pass.  Wrong arguments
 raise ``BoaError`` with ``BOA_E_INVALID``.
+
+The results carry no autograd graph.  A tensor that requires a gradient is
+refused where torch would record one (and so is a forward-mode dual), instead
+of cutting the graph in silence: call these inside ``torch.no_grad()``, from a
+``torch.autograd.Function`` whose backward is ``once_differentiable``, or on
+detached tensors.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import BOA_E_INVALID, BoaError, lib
 
@@ -34,6 +41,20 @@ def _raw_stream(index: int) -> int:
 
 # the same without the Stream object, which takes longer to make than a launch
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _no_graph(names, *tensors):
+    """Refuses tensors whose gradient would be lost."""
+    if torch.is_grad_enabled():
+        for i, t in enumerate(tensors):
+            if t is not None and t.requires_grad:
+                name = names.split()[i]
+                _bad(f"{name} requires a gradient, which the result would not carry: call inside torch.no_grad(), "
+                     f"from an autograd.Function (backward once_differentiable), or on {name}.detach()")
+    if forward_ad._current_level >= 0:
+        for i, t in enumerate(tensors):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _bad(f"{names.split()[i]} is a forward-mode dual, whose tangent the result would not carry")
 
 
 def _call(fn, index, *args):
@@ -115,6 +136,7 @@ def embed(tokens, table, scale: float = 1.0, dtype=None, out=None):
     """scale * table[tokens]: tokens of any shape (uint8, int32 or int64; one
     outside the table pads and gives a zero row), table [vocab <= 1024, d].
     -> tokens.shape + (d,) of `dtype` (the table's when not given)."""
+    _no_graph("table out", table, out)
     tokens, tok, index = _tokens(tokens)
     if table.dim() != 2:
         _bad("table must be [vocab, d]")
@@ -139,6 +161,7 @@ def embed_backward(tokens, dout, vocab: int, scale: float = 1.0, dtype=torch.flo
                    accumulate: bool = False):
     """Gradient of ``embed`` by its table, [vocab, d] of `dtype` (or in `out`,
     added to what it holds when `accumulate`)."""
+    _no_graph("dout out", dout, out)
     tokens, tok, index = _tokens(tokens)
     n = tokens.numel()
     if dout.dim() < 1 or dout.shape[-1] < 1 or dout.shape[:-1] != tokens.shape:
@@ -214,6 +237,7 @@ def mingru_scan(zh, h0=None, lengths=None, out=None, h_last=None, save_states: b
     nor part of the recurrence, and zero in h.  -> (h [chunks, positions, d],
     h_last fp32 [chunks, d]) and, with save_states, what
     ``mingru_scan_backward`` needs.  h_last may be h0 (updated in place)."""
+    _no_graph("zh h0 out h_last", zh, h0, out, h_last)
     zh, B, T, d, zr, zc, index = _gates(zh)
     out, hr, hc = _result(out, zh, (B, T, d), index, "out")
     h0 = _state(h0, (B, d), index, "h0")
@@ -233,6 +257,7 @@ def mingru_scan_backward(zh, states, dh, dh_last=None, lengths=None, out=None):
     """Gradient of ``mingru_scan`` from dh [chunks, positions, d] (zh's dtype)
     and dh_last fp32 [chunks, d] (None = zeros), with the states its forward
     call saved.  -> (dzh like zh, dh0 fp32 [chunks, d])"""
+    _no_graph("zh states dh dh_last out", zh, states, dh, dh_last, out)
     zh, B, T, d, zr, zc, index = _gates(zh)
     if dh.shape != (B, T, d) or dh.dtype != zh.dtype:
         _bad(f"dh must be {zh.dtype} of shape ({B}, {T}, {d})")
@@ -259,6 +284,7 @@ def token_loss(logits, targets, inv_temperature: float = 1.0, grad_scale: float 
     The gradient is formed when grad_scale, dloss or out is given: that of
     sum(grad_scale * dloss * loss), with dloss fp32 [...] (None = ones), in the
     logits' dtype, in `out` when given (which may be `logits`)."""
+    _no_graph("logits dloss out", logits, dloss, out)
     targets, tok, index = _tokens(targets, "targets")
     if logits.dim() < 1 or logits.shape[:-1] != targets.shape:
         _bad(f"logits {tuple(logits.shape)} do not match targets {tuple(targets.shape)}")

@@ -199,3 +199,40 @@ def test_a_wait_that_runs_out_gives_nan_and_nothing_else(tr, boa, silent):
     assert call(torch.cuda.current_stream().cuda_stream) == 0
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(outs, want))
+
+
+def test_wrapped_in_an_autograd_function(tr, boa):
+    """The recurrence as a differentiable function: its first derivative is
+    that of the calls, a second one is refused, not silently zero."""
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    class Cell(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, zh):
+            h, _, saved = tr.mingru_scan(zh, save_states=True)
+            ctx.save_for_backward(zh, saved)
+            return h
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, dh):
+            return tr.mingru_scan_backward(*ctx.saved_tensors, dh)[0]
+
+    class Unmarked(Cell):
+        @staticmethod
+        def backward(ctx, dh):
+            return tr.mingru_scan_backward(*ctx.saved_tensors, dh)[0]
+    zh = torch.randn(2, 50, 32, device="cuda", requires_grad=True)
+    dh = torch.randn(2, 50, 16, device="cuda")
+    with torch.no_grad():
+        _, _, saved = tr.mingru_scan(zh, save_states=True)
+        want = tr.mingru_scan_backward(zh, saved, dh)[0]
+    assert torch.equal(torch.autograd.grad(Cell.apply(zh), zh, dh)[0], want)
+    g, = torch.autograd.grad(Cell.apply(zh), zh, dh, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), zh)
+    with pytest.raises(boa.BoaError, match="zh requires a gradient"):
+        torch.autograd.grad(Unmarked.apply(zh), zh, dh, create_graph=True)
+    with pytest.raises(boa.BoaError, match="zh requires a gradient"):
+        tr.mingru_scan(zh)
