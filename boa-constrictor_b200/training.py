@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import BOA_E_INVALID, BoaError, lib
 
@@ -57,8 +58,10 @@ def _no_graph(names, *tensors):
                 _bad(f"{names.split()[i]} is a forward-mode dual, whose tangent the result would not carry")
 
 
-def _call(fn, index, *args):
-    """fn(*args, stream) with device `index` current, on torch's current stream of it."""
+def _call(fn, index, given, *args):
+    """fn(*args, stream) with device `index` current, on torch's current stream
+    of it.  `given`: the caller's tensors that it writes; torch is told that
+    they changed, so that a backward pass that saved one of them notices."""
     if index == torch.cuda.current_device():
         rc = fn(*args, _stream(index))
     else:
@@ -66,6 +69,9 @@ def _call(fn, index, *args):
             rc = fn(*args, _stream(index))
     if rc != 0:
         raise BoaError(rc, (lib().boa_last_error(None) or b"").decode())
+    for t in given:
+        if t is not None:
+            increment_version(t)
 
 
 def _same(index, t, name):
@@ -143,7 +149,7 @@ def embed(tokens, table, scale: float = 1.0, dtype=None, out=None):
     vocab, d = table.shape
     _same(index, table, "table")
     table, ld = _rows(table, vocab, d, "table")
-    n, shape = tokens.numel(), tokens.shape + (d,)
+    n, shape, given = tokens.numel(), tokens.shape + (d,), (out,)
     if out is None:
         out = table.new_empty(shape, dtype=dtype)
         rows, ld_out = out, d
@@ -152,8 +158,8 @@ def embed(tokens, table, scale: float = 1.0, dtype=None, out=None):
             _bad(f"out must be of shape {tuple(shape)} and of dtype {dtype or out.dtype}")
         _same(index, out, "out")
         rows, ld_out = _rows(out, n, d, "out", write=True)
-    _call(lib().boa_embed, index, tokens.data_ptr(), tok, n, table.data_ptr(), _type(table, "table"), ld, vocab, d,
-          scale, rows.data_ptr(), _type(out, "out"), ld_out)
+    _call(lib().boa_embed, index, given, tokens.data_ptr(), tok, n, table.data_ptr(), _type(table, "table"), ld, vocab,
+          d, scale, rows.data_ptr(), _type(out, "out"), ld_out)
     return out
 
 
@@ -169,6 +175,7 @@ def embed_backward(tokens, dout, vocab: int, scale: float = 1.0, dtype=torch.flo
     d = dout.shape[-1]
     _same(index, dout, "dout")
     dout, ld = _rows(dout, n, d, "dout")
+    given = (out,)
     if out is None:
         if accumulate:
             _bad("accumulate needs out")
@@ -184,8 +191,8 @@ def embed_backward(tokens, dout, vocab: int, scale: float = 1.0, dtype=torch.flo
     L = lib()
     need = L.boa_embed_backward_workspace(n, vocab, d)
     ws = tokens.new_empty(need, dtype=torch.uint8) if need else None
-    _call(L.boa_embed_backward, index, tokens.data_ptr(), tok, n, dout.data_ptr(), _type(dout, "dout"), ld, vocab, d,
-          scale, int(accumulate), rows.data_ptr(), _type(out, "out"), ld_out, _ptr(ws), need)
+    _call(L.boa_embed_backward, index, given, tokens.data_ptr(), tok, n, dout.data_ptr(), _type(dout, "dout"), ld,
+          vocab, d, scale, int(accumulate), rows.data_ptr(), _type(out, "out"), ld_out, _ptr(ws), need)
     return out
 
 
@@ -239,6 +246,7 @@ def mingru_scan(zh, h0=None, lengths=None, out=None, h_last=None, save_states: b
     ``mingru_scan_backward`` needs.  h_last may be h0 (updated in place)."""
     _no_graph("zh h0 out h_last", zh, h0, out, h_last)
     zh, B, T, d, zr, zc, index = _gates(zh)
+    given = (out, h_last)
     out, hr, hc = _result(out, zh, (B, T, d), index, "out")
     h0 = _state(h0, (B, d), index, "h0")
     if h_last is None:
@@ -248,7 +256,7 @@ def mingru_scan(zh, h0=None, lengths=None, out=None, h_last=None, save_states: b
     lengths = _lengths(lengths, B, index)
     L = lib()
     states = zh.new_empty(L.boa_mingru_states_floats(B, T, d), dtype=_FLOAT) if save_states else None
-    _call(L.boa_mingru_scan, index, zh.data_ptr(), _type(zh, "zh"), zr, zc, B, T, d, _ptr(lengths), _ptr(h0),
+    _call(L.boa_mingru_scan, index, given, zh.data_ptr(), _type(zh, "zh"), zr, zc, B, T, d, _ptr(lengths), _ptr(h0),
           out.data_ptr(), hr, hc, h_last.data_ptr(), _ptr(states))
     return (out, h_last, states) if save_states else (out, h_last)
 
@@ -267,11 +275,12 @@ def mingru_scan_backward(zh, states, dh, dh_last=None, lengths=None, out=None):
     if states.dtype != _FLOAT or states.numel() != L.boa_mingru_states_floats(B, T, d) or not states.is_contiguous():
         _bad("states must be what mingru_scan(..., save_states=True) returned for these sizes")
     _same(index, states, "states")
+    given = (out,)
     out, dr, dc = _result(out, zh, (B, T, 2 * d), index, "out")
     dh_last = _state(dh_last, (B, d), index, "dh_last")
     dh0 = zh.new_empty((B, d), dtype=_FLOAT)
     lengths = _lengths(lengths, B, index)
-    _call(L.boa_mingru_scan_backward, index, zh.data_ptr(), _type(zh, "zh"), zr, zc, B, T, d, _ptr(lengths),
+    _call(L.boa_mingru_scan_backward, index, given, zh.data_ptr(), _type(zh, "zh"), zr, zc, B, T, d, _ptr(lengths),
           states.data_ptr(), dh.data_ptr(), gr, gc, _ptr(dh_last), out.data_ptr(), dr, dc, dh0.data_ptr())
     return out, dh0
 
@@ -292,7 +301,7 @@ def token_loss(logits, targets, inv_temperature: float = 1.0, grad_scale: float 
     _same(index, logits, "logits")
     rows, ld = _rows(logits, n, vocab, "logits")
     loss = targets.new_empty(targets.shape, dtype=_FLOAT)
-    grad, ld_grad = None, 0
+    grad, ld_grad, given = None, 0, (out,)
     if dloss is not None:
         if dloss.get_device() != index or dloss.dtype != _FLOAT or dloss.shape != targets.shape:
             _bad(f"dloss must be float32 of shape {tuple(targets.shape)} on cuda:{index}")
@@ -307,7 +316,7 @@ def token_loss(logits, targets, inv_temperature: float = 1.0, grad_scale: float 
     elif grad_scale is not None or dloss is not None:
         out = grad = logits.new_empty(logits.shape)
         ld_grad = vocab
-    _call(lib().boa_token_loss, index, rows.data_ptr(), _type(logits, "logits"), ld, n, vocab, targets.data_ptr(),
-          tok, inv_temperature, _ptr(dloss), 1.0 if grad_scale is None else grad_scale, loss.data_ptr(), _ptr(grad),
+    _call(lib().boa_token_loss, index, given, rows.data_ptr(), _type(logits, "logits"), ld, n, vocab,
+          targets.data_ptr(), tok, inv_temperature, _ptr(dloss), 1.0 if grad_scale is None else grad_scale, loss.data_ptr(), _ptr(grad),
           ld_grad)
     return loss, out

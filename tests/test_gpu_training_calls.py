@@ -236,3 +236,36 @@ def test_wrapped_in_an_autograd_function(tr, boa):
         torch.autograd.grad(Unmarked.apply(zh), zh, dh, create_graph=True)
     with pytest.raises(boa.BoaError, match="zh requires a gradient"):
         tr.mingru_scan(zh)
+
+
+def _writers(tr, torch):
+    r = lambda *s: torch.randn(*s, device="cuda")  # noqa: E731
+    tok = torch.randint(0, 8, (6,), device="cuda")
+    zh, h0 = r(2, 5, 8), r(2, 4)
+    saved = tr.mingru_scan(zh, h0, save_states=True)[2]
+    return {
+        "embed": ((6, 4), lambda y: tr.embed(tok, r(8, 4), out=y)),
+        "embed_backward": ((8, 4), lambda y: tr.embed_backward(tok, r(6, 4), 8, out=y)),
+        "accumulate": ((8, 4), lambda y: tr.embed_backward(tok, r(6, 4), 8, out=y, accumulate=True)),
+        "scan": ((2, 5, 4), lambda y: tr.mingru_scan(zh, h0, out=y)),
+        "state": ((2, 4), lambda y: tr.mingru_scan(zh, y, h_last=y)),
+        "scan_backward": ((2, 5, 8), lambda y: tr.mingru_scan_backward(zh, saved, r(2, 5, 4), out=y)),
+        "loss": ((6, 8), lambda y: tr.token_loss(y, tok, out=y)),
+    }
+
+
+@pytest.mark.parametrize("name", ["embed", "embed_backward", "accumulate", "scan", "state", "scan_backward", "loss"])
+def test_a_saved_tensor_that_is_written_is_noticed(tr, name):
+    """exp saves its result for its gradient: written over by one of these
+    calls, torch refuses the backward pass, as after an in-place operation."""
+    import torch
+    shape, write = _writers(tr, torch)[name]
+    a = torch.randn(shape, device="cuda", requires_grad=True)
+    y = a.exp()
+    write(y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():  # tensors without versions are written all the same
+        z = torch.full(shape, 0.5, device="cuda")
+        write(z)
+        assert not (z == 0.5).all()
