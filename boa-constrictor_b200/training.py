@@ -95,6 +95,15 @@ def _tokens(tokens, name="tokens"):
     return (tokens if tokens.is_contiguous() else tokens.contiguous()), k, index
 
 
+def _sign(x, name, write=False):
+    """x as it reads in memory: the imaginary part of a conjugate is a view whose sign torch keeps aside"""
+    if x.is_neg():
+        if write:
+            _bad(f"{name} must not be a negative view")
+        return x.resolve_neg()
+    return x
+
+
 def _rows(x, n, width, name, write=False):
     """x as n rows of `width` -> (tensor that holds them, elements between
     rows).  Rows that no single stride reaches are copied, unless they are
@@ -102,6 +111,7 @@ def _rows(x, n, width, name, write=False):
     shape = x.shape
     if not shape or shape[-1] != width or x.numel() != n * width:
         _bad(f"{name} has shape {tuple(shape)}, not {n} rows of {width}")
+    x = _sign(x, name, write)
     if x.is_contiguous():
         return x, width
     rows = x
@@ -129,6 +139,7 @@ def _state(x, shape, index, name, write=False):
         return None
     if x.get_device() != index or x.dtype != _FLOAT or x.shape != shape:
         _bad(f"{name} must be float32 of shape {shape} on cuda:{index}")
+    x = _sign(x, name, write)
     if x.is_contiguous():
         return x
     return _bad(f"{name} must be contiguous") if write else x.contiguous()
@@ -210,6 +221,7 @@ def _gates(zh):
 
 def _steps(x, name, write=False):
     """x with contiguous rows -> (x, elements between positions, between chunks)"""
+    x = _sign(x, name, write)
     chunk, row, one = x.stride()
     if one == 1 or x.shape[2] == 1:
         return x, row, chunk
@@ -305,7 +317,7 @@ def token_loss(logits, targets, inv_temperature: float = 1.0, grad_scale: float 
     if dloss is not None:
         if dloss.get_device() != index or dloss.dtype != _FLOAT or dloss.shape != targets.shape:
             _bad(f"dloss must be float32 of shape {tuple(targets.shape)} on cuda:{index}")
-        dloss = dloss.contiguous()
+        dloss = _sign(dloss, "dloss").contiguous()
     if out is not None:
         if out.shape != logits.shape or out.dtype != logits.dtype:
             _bad(f"out must be {logits.dtype} of shape {tuple(logits.shape)}")
@@ -317,6 +329,6 @@ def token_loss(logits, targets, inv_temperature: float = 1.0, grad_scale: float 
         out = grad = logits.new_empty(logits.shape)
         ld_grad = vocab
     _call(lib().boa_token_loss, index, given, rows.data_ptr(), _type(logits, "logits"), ld, n, vocab,
-          targets.data_ptr(), tok, inv_temperature, _ptr(dloss), 1.0 if grad_scale is None else grad_scale, loss.data_ptr(), _ptr(grad),
-          ld_grad)
+          targets.data_ptr(), tok, inv_temperature, _ptr(dloss), 1.0 if grad_scale is None else grad_scale,
+          loss.data_ptr(), _ptr(grad), ld_grad)
     return loss, out

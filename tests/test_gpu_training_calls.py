@@ -269,3 +269,28 @@ def test_a_saved_tensor_that_is_written_is_noticed(tr, name):
         z = torch.full(shape, 0.5, device="cuda")
         write(z)
         assert not (z == 0.5).all()
+
+
+def _negative(torch, *shape):
+    """A real view whose sign torch keeps aside, and the same values in memory."""
+    x = torch.view_as_complex(torch.randn(*shape, 2, device="cuda")).conj().imag
+    assert x.is_neg()
+    return x, x.clone().resolve_neg()
+
+
+def test_negative_views_keep_their_sign(tr, boa):
+    import torch
+    tok = torch.randint(0, 8, (6,), device="cuda")
+    t, h0, dl, w = (_negative(torch, *s) for s in ((8, 4), (2, 4), (2, 4), (6,)))
+    x, zh, dh, g = (_negative(torch, *s) for s in ((6, 8), (2, 5, 8), (2, 5, 4), (6, 4)))
+    saved = tr.mingru_scan(zh[1], h0[1], save_states=True)[2]
+    both = [[tr.embed(tok, t[k]), tr.embed_backward(tok, g[k], 8), *tr.mingru_scan(zh[k], h0[k]),
+             *tr.mingru_scan_backward(zh[k], saved, dh[k], dl[k]), *tr.token_loss(x[k], tok, dloss=w[k])] for k in (0, 1)]
+    for a, b in zip(*both):
+        assert not a.is_neg() and torch.equal(a, b)
+    for write in (lambda: tr.embed(tok, t[1], out=g[0]), lambda: tr.embed_backward(tok, g[1], 8, out=t[0]),
+                  lambda: tr.mingru_scan(zh[1], out=dh[0]), lambda: tr.mingru_scan(zh[1], h_last=h0[0]),
+                  lambda: tr.mingru_scan_backward(zh[1], saved, dh[1], out=zh[0]),
+                  lambda: tr.token_loss(x[1], tok, out=x[0])):
+        with pytest.raises(boa.BoaError, match="negative view"):
+            write()
