@@ -30,10 +30,14 @@ from . import BOA_E_INVALID, BoaError, lib
 _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _TOKEN = {torch.uint8: 0, torch.int32: 1, torch.int64: 2}
 _FLOAT = torch.float32
+_INT = 0x7FFFFFFF  # the largest C int: of a larger size ctypes would pass the low half
 
 
 def _bad(what: str):
     raise BoaError(BOA_E_INVALID, what)
+
+
+_grad_on = torch.is_grad_enabled
 
 
 def _raw_stream(index: int) -> int:
@@ -42,27 +46,35 @@ def _raw_stream(index: int) -> int:
 
 # the same without the Stream object, which takes longer to make than a launch
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+# and the device without the check that CUDA is initialised: the tensors are on a GPU already
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _no_graph(names, *tensors):
     """Refuses tensors whose gradient would be lost."""
-    if torch.is_grad_enabled():
-        for i, t in enumerate(tensors):
+    if _grad_on():
+        for t in tensors:
             if t is not None and t.requires_grad:
-                name = names.split()[i]
+                name = names.split()[[t is x for x in tensors].index(True)]
                 _bad(f"{name} requires a gradient, which the result would not carry: call inside torch.no_grad(), "
                      f"from an autograd.Function (backward once_differentiable), or on {name}.detach()")
     if forward_ad._current_level >= 0:
-        for i, t in enumerate(tensors):
+        for name, t in zip(names.split(), tensors):
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                _bad(f"{names.split()[i]} is a forward-mode dual, whose tangent the result would not carry")
+                _bad(f"{name} is a forward-mode dual, whose tangent the result would not carry")
+
+
+def _given(out, state=None):
+    if state is None:
+        return () if out is None else (out,)
+    return (state,) if out is None else (out, state)
 
 
 def _call(fn, index, given, *args):
     """fn(*args, stream) with device `index` current, on torch's current stream
     of it.  `given`: the caller's tensors that it writes; torch is told that
     they changed, so that a backward pass that saved one of them notices."""
-    if index == torch.cuda.current_device():
+    if index == _device():
         rc = fn(*args, _stream(index))
     else:
         with torch.cuda.device(index):
@@ -70,8 +82,7 @@ def _call(fn, index, given, *args):
     if rc != 0:
         raise BoaError(rc, (lib().boa_last_error(None) or b"").decode())
     for t in given:
-        if t is not None:
-            increment_version(t)
+        increment_version(t)
 
 
 def _same(index, t, name):
@@ -96,12 +107,11 @@ def _tokens(tokens, name="tokens"):
 
 
 def _sign(x, name, write=False):
-    """x as it reads in memory: the imaginary part of a conjugate is a view whose sign torch keeps aside"""
-    if x.is_neg():
-        if write:
-            _bad(f"{name} must not be a negative view")
-        return x.resolve_neg()
-    return x
+    """A negative view (the imaginary part of a conjugate, whose sign torch
+    keeps aside) as it reads in memory."""
+    if write:
+        _bad(f"{name} must not be a negative view")
+    return x.resolve_neg()
 
 
 def _rows(x, n, width, name, write=False):
@@ -111,7 +121,8 @@ def _rows(x, n, width, name, write=False):
     shape = x.shape
     if not shape or shape[-1] != width or x.numel() != n * width:
         _bad(f"{name} has shape {tuple(shape)}, not {n} rows of {width}")
-    x = _sign(x, name, write)
+    if x.is_neg():
+        x = _sign(x, name, write)
     if x.is_contiguous():
         return x, width
     rows = x
@@ -139,7 +150,8 @@ def _state(x, shape, index, name, write=False):
         return None
     if x.get_device() != index or x.dtype != _FLOAT or x.shape != shape:
         _bad(f"{name} must be float32 of shape {shape} on cuda:{index}")
-    x = _sign(x, name, write)
+    if x.is_neg():
+        x = _sign(x, name, write)
     if x.is_contiguous():
         return x
     return _bad(f"{name} must be contiguous") if write else x.contiguous()
@@ -158,9 +170,11 @@ def embed(tokens, table, scale: float = 1.0, dtype=None, out=None):
     if table.dim() != 2:
         _bad("table must be [vocab, d]")
     vocab, d = table.shape
+    if vocab > _INT or d > _INT:
+        _bad("the sides of table must be below 2^31")
     _same(index, table, "table")
     table, ld = _rows(table, vocab, d, "table")
-    n, shape, given = tokens.numel(), tokens.shape + (d,), (out,)
+    n, shape, given = tokens.numel(), tokens.shape + (d,), _given(out)
     if out is None:
         out = table.new_empty(shape, dtype=dtype)
         rows, ld_out = out, d
@@ -184,9 +198,11 @@ def embed_backward(tokens, dout, vocab: int, scale: float = 1.0, dtype=torch.flo
     if dout.dim() < 1 or dout.shape[-1] < 1 or dout.shape[:-1] != tokens.shape:
         _bad(f"dout must be of shape {tuple(tokens.shape)} + (d,), not {tuple(dout.shape)}")
     d = dout.shape[-1]
+    if vocab > _INT or d > _INT:
+        _bad("vocab and d must be below 2^31")
     _same(index, dout, "dout")
     dout, ld = _rows(dout, n, d, "dout")
-    given = (out,)
+    given = _given(out)
     if out is None:
         if accumulate:
             _bad("accumulate needs out")
@@ -215,13 +231,16 @@ def _gates(zh):
     B, T, w = zh.shape
     if w < 2 or w % 2:
         _bad("zh must be a CUDA tensor [chunks, positions, 2 d]")
+    if B > _INT or T > _INT or w > _INT:
+        _bad("chunks, positions and 2 d must be below 2^31")
     zh, row, chunk = _steps(zh, "zh")
     return zh, B, T, w // 2, row, chunk, index
 
 
 def _steps(x, name, write=False):
     """x with contiguous rows -> (x, elements between positions, between chunks)"""
-    x = _sign(x, name, write)
+    if x.is_neg():
+        x = _sign(x, name, write)
     chunk, row, one = x.stride()
     if one == 1 or x.shape[2] == 1:
         return x, row, chunk
@@ -258,7 +277,7 @@ def mingru_scan(zh, h0=None, lengths=None, out=None, h_last=None, save_states: b
     ``mingru_scan_backward`` needs.  h_last may be h0 (updated in place)."""
     _no_graph("zh h0 out h_last", zh, h0, out, h_last)
     zh, B, T, d, zr, zc, index = _gates(zh)
-    given = (out, h_last)
+    given = _given(out, h_last)
     out, hr, hc = _result(out, zh, (B, T, d), index, "out")
     h0 = _state(h0, (B, d), index, "h0")
     if h_last is None:
@@ -287,7 +306,7 @@ def mingru_scan_backward(zh, states, dh, dh_last=None, lengths=None, out=None):
     if states.dtype != _FLOAT or states.numel() != L.boa_mingru_states_floats(B, T, d) or not states.is_contiguous():
         _bad("states must be what mingru_scan(..., save_states=True) returned for these sizes")
     _same(index, states, "states")
-    given = (out,)
+    given = _given(out)
     out, dr, dc = _result(out, zh, (B, T, 2 * d), index, "out")
     dh_last = _state(dh_last, (B, d), index, "dh_last")
     dh0 = zh.new_empty((B, d), dtype=_FLOAT)
@@ -310,14 +329,16 @@ def token_loss(logits, targets, inv_temperature: float = 1.0, grad_scale: float 
     if logits.dim() < 1 or logits.shape[:-1] != targets.shape:
         _bad(f"logits {tuple(logits.shape)} do not match targets {tuple(targets.shape)}")
     n, vocab = targets.numel(), logits.shape[-1]
+    if vocab > _INT:
+        _bad("vocab must be below 2^31")
     _same(index, logits, "logits")
     rows, ld = _rows(logits, n, vocab, "logits")
     loss = targets.new_empty(targets.shape, dtype=_FLOAT)
-    grad, ld_grad, given = None, 0, (out,)
+    grad, ld_grad, given = None, 0, _given(out)
     if dloss is not None:
         if dloss.get_device() != index or dloss.dtype != _FLOAT or dloss.shape != targets.shape:
             _bad(f"dloss must be float32 of shape {tuple(targets.shape)} on cuda:{index}")
-        dloss = _sign(dloss, "dloss").contiguous()
+        dloss = dloss.resolve_neg().contiguous()
     if out is not None:
         if out.shape != logits.shape or out.dtype != logits.dtype:
             _bad(f"out must be {logits.dtype} of shape {tuple(logits.shape)}")

@@ -294,3 +294,23 @@ def test_negative_views_keep_their_sign(tr, boa):
                   lambda: tr.token_loss(x[1], tok, out=x[0])):
         with pytest.raises(boa.BoaError, match="negative view"):
             write()
+
+
+def test_sizes_past_a_c_int_are_refused(tr, boa):
+    """Not taken by their low halves.  Views of one element, and of none."""
+    import torch
+    far = (1 << 32) + 8
+    tok, one = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(1, 1, device="cuda")
+    none = torch.zeros(1, 0, 2, device="cuda")
+    h0 = torch.zeros(1, 1, device="cuda")
+    for call in (lambda: tr.embed(tok, one.expand(far, 1)), lambda: tr.embed(tok[:0], one.expand(1, far)),
+                 lambda: tr.embed_backward(tok, torch.zeros(4, 1, device="cuda"), far),
+                 lambda: tr.embed_backward(tok[:0], torch.zeros(0, 1, device="cuda").expand(0, far), 1),
+                 lambda: tr.mingru_scan(none.expand(far, 0, 2)),
+                 lambda: tr.mingru_scan(one[None].half().expand(1, far, 2)),
+                 lambda: tr.mingru_scan_backward(none.expand(far, 0, 2), none, none.expand(far, 0, 2)[..., :1], h0),
+                 lambda: tr.token_loss(torch.zeros(0, 1, device="cuda").expand(0, far), tok[:0])):
+        before = torch.cuda.memory_allocated()
+        with pytest.raises(boa.BoaError, match="below 2"):
+            call()
+        assert torch.cuda.memory_allocated() == before
