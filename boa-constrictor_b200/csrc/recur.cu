@@ -706,6 +706,9 @@ cudaError_t launch_walk_selftest(int steps, int silent, uint64_t limit_ns, float
 // ------------------------------------------------------------- few positions
 // Up to kFew positions (the decode step): a thread takes V chains through
 // all of them, all loads issued first.
+// The cell and the state's update are the same operations for every V, T_ and
+// STEPS, so that any cut of a sequence into such calls gives the same bits:
+// the header promises that, for an encoder and a decoder that must agree.
 template <typename T_, int V, int STEPS>
 __global__ void __launch_bounds__(256)
 mingru_step_kernel(const T_* __restrict__ zh, RowStrides zs, int T, int d, FastDiv by_d, long long chains,

@@ -274,7 +274,11 @@ def mingru_scan(zh, h0=None, lengths=None, out=None, h_last=None, save_states: b
     lengths: int32 positions of each chunk; rows past them are neither read
     nor part of the recurrence, and zero in h.  -> (h [chunks, positions, d],
     h_last fp32 [chunks, d]) and, with save_states, what
-    ``mingru_scan_backward`` needs.  h_last may be h0 (updated in place)."""
+    ``mingru_scan_backward`` needs.  h_last may be h0 (updated in place).
+
+    Calls of up to 8 positions give the same bits however a sequence is cut
+    into them; a longer one agrees with them to rounding only.  An encoder and
+    a decoder that must agree both step in calls of at most 8."""
     _no_graph("zh h0 out h_last", zh, h0, out, h_last)
     zh, B, T, d, zr, zc, index = _gates(zh)
     given = _given(out, h_last)

@@ -258,8 +258,9 @@ int boa_cdf_from_logits(boa_model* h, const float* logits, int rows, float inv_t
  * Element types (BOA_F32 ..) may differ where an argument names its own type;
  * arithmetic is fp32 or wider and results are rounded once, to nearest.
  * Buffers need the alignment of their element only; 16-byte aligned buffers
- * and rows run fastest.  Results do not depend on timing: the same inputs on
- * the same kind of GPU give the same bits. */
+ * and rows run fastest.  Results do not depend on timing: the same call (its
+ * values, sizes, strides and alignment) on the same kind of GPU gives the same
+ * bits.  Another size, stride or alignment may sum in another order. */
 #define BOA_F32 0
 #define BOA_F16 1
 #define BOA_BF16 2
@@ -296,7 +297,15 @@ int boa_embed_backward(const void* d_tokens, int token_type, int64_t n, const vo
  * boa_mingru_states_floats floats that the backward call needs; their layout
  * is the library's own.  T = 0 only moves the state.  A gate logit below -88
  * counts as closed (z = 0); NaN in a row makes the chain's states from there
- * on, and its gradients, NaN. */
+ * on, and its gradients, NaN.
+ * Which calls agree bit by bit: up to 8 positions are taken in order, so a
+ * sequence cut into calls of 1 to 8 positions has the same h and the same
+ * states however it is cut, however many chunks go together and whatever
+ * their strides and alignment.  A longer call joins parts of the sequence, in
+ * an order that depends on its sizes, strides and alignment and on the GPU:
+ * its results differ from those, and from another long call's, in the last
+ * bits.  An encoder and a decoder that must agree on the bits (a coder's model
+ * must) both step in calls of at most 8 positions. */
 uint64_t boa_mingru_states_floats(int n_chunks, int T, int d);
 int boa_mingru_scan(const void* d_zh, int type, int64_t zh_row, int64_t zh_chunk, int n_chunks, int T, int d,
                     const int32_t* d_lengths, const float* d_h0, void* d_h, int64_t h_row, int64_t h_chunk,
