@@ -902,12 +902,15 @@ cudaError_t launch_mingru_scan(const void* zh, int type, RowStrides zs, int B, i
       return launch_walk<kernel>(s, st, x, zs, T, d, by_d, chains, lengths, h0, o, hs, h_last, states);
     };
     // two chains a lane: always for 16 bits; for 32 bits where that leaves
-    // groups enough to fill the GPU
+    // groups enough to fill the GPU.  (16 bytes a lane mean 16-bit pairs, so
+    // 16-bit single chains never go with them.)
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;
     if (pairs && (sizeof(E) == 2 || T <= kFew || chains >= 148 * 64))
       return quads && T > kFew ? go(two, std::true_type{}) : go(two, std::false_type{});
-    return sizeof(E) == 4 && quads ? go(one, std::true_type{}) : go(one, std::false_type{});
+    if constexpr (sizeof(E) == 4)
+      if (quads) return go(one, std::true_type{});
+    return go(one, std::false_type{});
   });
 }
 
@@ -945,8 +948,12 @@ cudaError_t launch_mingru_scan_grad(const void* zh, int type, RowStrides zs, int
     };
     constexpr std::integral_constant<int, 1> one;
     constexpr std::integral_constant<int, 2> two;
-    if (pairs && sizeof(E) == 2) return quads ? go(two, std::true_type{}) : go(two, std::false_type{});
-    return sizeof(E) == 4 && quads ? go(one, std::true_type{}) : go(one, std::false_type{});
+    if constexpr (sizeof(E) == 2) {
+      if (pairs) return quads ? go(two, std::true_type{}) : go(two, std::false_type{});
+    } else {
+      if (quads) return go(one, std::true_type{});
+    }
+    return go(one, std::false_type{});
   });
 }
 
