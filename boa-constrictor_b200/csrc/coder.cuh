@@ -16,7 +16,7 @@
 // update (:765-780).  Pure integer arithmetic -> bit-exact.
 #pragma once
 #include <cstdint>
-#include "ptx.cuh"
+#include "devword.cuh"
 
 namespace boa {
 

@@ -18,7 +18,6 @@
 // Measured on a B200: 1M x 256 fp32 lookup 148 us (7.2 TB/s of stores); its
 // gradient 191 us; profiled one by one, the row sums take 169 us (6.4 TB/s) and
 // the sort's three launches 28 us.
-#include "kernels.cuh"
 #include "pieces.h"
 #include "ptx.cuh"
 #include "train_ops.cuh"

@@ -15,8 +15,6 @@
 // (32 lanes: 376 us and 258 us).
 #include <cfloat>
 
-#include "kernels.cuh"
-#include "ptx.cuh"
 #include "train_ops.cuh"
 
 namespace boa {

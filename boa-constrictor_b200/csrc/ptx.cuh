@@ -1,10 +1,8 @@
 // ptx.cuh -- thin inline-PTX wrappers for sm_100a: mbarriers, TMA bulk-tensor
 // loads, tcgen05 (TMEM alloc, UMMA issue/commit, TMEM loads) and bounded waits.
 //
-// Every wait is bounded by the global nanosecond timer.  A wait that runs out
-// records BOA_ERR_TIMEOUT in the device error word and returns false, so a
-// kernel can skip its remaining work, release its TMEM and exit instead of
-// hanging the GPU.
+// Every wait of this library is bounded by the global nanosecond timer.  The
+// waits that record a timeout in the device error word are in devword.cuh.
 #pragma once
 #include <cstdint>
 #include <cuda.h>
@@ -12,14 +10,6 @@
 #include <cuda_bf16.h>
 
 namespace boa {
-
-// device error word (read by the host after each synchronising call)
-enum : int { BOA_ERR_NONE = 0, BOA_ERR_TIMEOUT = 1, BOA_ERR_STREAM_OVERFLOW = 2, BOA_ERR_BAD_INPUT = 3 };
-// One definition: the library is built as a single translation unit
-// (csrc/boa_all.cu), so device and host code see the same symbol.
-__device__ int g_dev_error = 0;
-
-__device__ __forceinline__ void set_dev_error(int code) { atomicCAS(&g_dev_error, 0, code); }
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s per wait
 
@@ -58,25 +48,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait for the phase with the given parity to complete: past the
-// limit it records BOA_ERR_TIMEOUT in the device error word and returns false,
-// and the caller unwinds without touching the barrier's data.
-__device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
-  const uint32_t a = smem_u32(bar);
-  if (mbar_try_wait(a, parity)) return true;
-  const uint64_t t0 = global_ns();
-  while (true) {
-    if (mbar_try_wait(a, parity)) return true;
-    if (global_ns() - t0 > limit_ns) {
-      set_dev_error(BOA_ERR_TIMEOUT);
-      return false;
-    }
-  }
-}
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
-  return mbar_wait_for(bar, parity, kWaitLimitNs);
-}
-
 // named barrier over a subset of warps (ids 1..15; id 0 is __syncthreads)
 __device__ __forceinline__ void named_bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");

@@ -35,7 +35,6 @@
 // Few chains are paced by the SMs that clusters reach: 1 x 262144 x 512 fp32
 // 392 us (0.63) and 673 us (0.61).  One position, 16384 x 256: 13.8 and 14.4 us
 // in two captures (0.93, 0.89).
-#include "kernels.cuh"
 #include "ptx.cuh"
 #include "train_ops.cuh"
 
