@@ -450,7 +450,8 @@ struct boa_pyrc {
 
 namespace {
 int pyrc_fail(boa_pyrc* h, int code, const std::string& msg) {
-  if (h) h->err = msg; else g_load_error = msg;
+  if (!h) return fail(nullptr, code, msg);
+  h->err = msg;
   return code;
 }
 int pyrc_cuda(boa_pyrc* h, cudaError_t e, const char* where) {

@@ -60,3 +60,13 @@ def test_a_tangent_is_not_dropped_in_silence(boa, op, name):
         with torch.no_grad(), pytest.raises(boa.BoaError, match=f"{name} is a forward-mode dual") as e:
             call(**args)
     assert e.value.code == boa.BOA_E_INVALID
+
+
+def test_a_later_failure_of_the_probability_coder_is_the_last_one(boa):
+    """boa_last_error(NULL) gives the last failed call without a handle, whichever kind it was."""
+    L = boa.lib()
+    assert L.boa_embed(None, 9, 0, None, 0, 0, 0, 0, 1.0, None, 0, 0, None) == boa.BOA_E_INVALID
+    assert L.boa_last_error(None).startswith(b"boa_embed")
+    h = C.c_void_p()
+    assert L.boa_pyrc_create(0, 4, 4, 0, C.byref(h)) == boa.BOA_E_INVALID
+    assert b"n_streams" in L.boa_last_error(None) and b"n_streams" in L.boa_pyrc_last_error(None)
