@@ -145,7 +145,7 @@ __device__ __forceinline__ Cell<V> mingru_cell(const Vec<V>& zl, const Vec<V>& h
     // hr + 1/2 lies below sigmoid(hr) for hr < 0 (slopes 1 and at most 1/4
     // from the same value at 0), and above sigmoid(-hr) <= 1/2 otherwise
     const float c = fmaxf(hr.v[v] + 0.5f, low);
-    k.a.v[v] = e <= 1.f ? e * z : 1.f - z;
+    k.a.v[v] = zl.v[v] >= 0.f ? e * z : 1.f - z;
     k.b.v[v] = z * c;
     k.z.v[v] = z;
     if (GRAD) k.w.v[v] = z * (hr.v[v] >= 0.f ? 1.f : __fmaf_rn(-low, low, low));
