@@ -37,9 +37,6 @@ def _bad(what: str):
     raise BoaError(BOA_E_INVALID, what)
 
 
-_grad_on = torch.is_grad_enabled
-
-
 def _raw_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
@@ -52,28 +49,20 @@ _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 def _no_graph(names, *tensors):
     """Refuses tensors whose gradient would be lost."""
-    if _grad_on():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                name = names.split()[[t is x for x in tensors].index(True)]
-                _bad(f"{name} requires a gradient, which the result would not carry: call inside torch.no_grad(), "
-                     f"from an autograd.Function (backward once_differentiable), or on {name}.detach()")
-    if forward_ad._current_level >= 0:
-        for name, t in zip(names.split(), tensors):
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                _bad(f"{name} is a forward-mode dual, whose tangent the result would not carry")
-
-
-def _given(out, state=None):
-    if state is None:
-        return () if out is None else (out,)
-    return (state,) if out is None else (out, state)
+    for name, t in zip(names.split(), tensors):
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
+            _bad(f"{name} requires a gradient, which the result would not carry: call inside torch.no_grad(), "
+                 f"from an autograd.Function (backward once_differentiable), or on {name}.detach()")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            _bad(f"{name} is a forward-mode dual, whose tangent the result would not carry")
 
 
 def _call(fn, index, given, *args):
     """fn(*args, stream) with device `index` current, on torch's current stream
-    of it.  `given`: the caller's tensors that it writes; torch is told that
-    they changed, so that a backward pass that saved one of them notices."""
+    of it.  `given`: the caller's tensor that it writes, or None; torch is told
+    that it changed, so that a backward pass that saved it notices."""
     if index == _device():
         rc = fn(*args, _stream(index))
     else:
@@ -81,8 +70,8 @@ def _call(fn, index, given, *args):
             rc = fn(*args, _stream(index))
     if rc != 0:
         raise BoaError(rc, (lib().boa_last_error(None) or b"").decode())
-    for t in given:
-        increment_version(t)
+    if given is not None:
+        increment_version(given)
 
 
 def _same(index, t, name):
@@ -165,7 +154,8 @@ def embed(tokens, table, scale: float = 1.0, dtype=None, out=None):
     """scale * table[tokens]: tokens of any shape (uint8, int32 or int64; one
     outside the table pads and gives a zero row), table [vocab <= 1024, d].
     -> tokens.shape + (d,) of `dtype` (the table's when not given)."""
-    _no_graph("table out", table, out)
+    if table.requires_grad or (out is not None and out.requires_grad) or forward_ad._current_level >= 0:
+        _no_graph("table out", table, out)
     tokens, tok, index = _tokens(tokens)
     if table.dim() != 2:
         _bad("table must be [vocab, d]")
@@ -174,7 +164,7 @@ def embed(tokens, table, scale: float = 1.0, dtype=None, out=None):
         _bad("the sides of table must be below 2^31")
     _same(index, table, "table")
     table, ld = _rows(table, vocab, d, "table")
-    n, shape, given = tokens.numel(), tokens.shape + (d,), _given(out)
+    n, shape, given = tokens.numel(), tokens.shape + (d,), out
     if out is None:
         out = table.new_empty(shape, dtype=dtype)
         rows, ld_out = out, d
@@ -192,7 +182,8 @@ def embed_backward(tokens, dout, vocab: int, scale: float = 1.0, dtype=torch.flo
                    accumulate: bool = False):
     """Gradient of ``embed`` by its table, [vocab, d] of `dtype` (or in `out`,
     added to what it holds when `accumulate`)."""
-    _no_graph("dout out", dout, out)
+    if dout.requires_grad or (out is not None and out.requires_grad) or forward_ad._current_level >= 0:
+        _no_graph("dout out", dout, out)
     tokens, tok, index = _tokens(tokens)
     n = tokens.numel()
     if dout.dim() < 1 or dout.shape[-1] < 1 or dout.shape[:-1] != tokens.shape:
@@ -202,7 +193,7 @@ def embed_backward(tokens, dout, vocab: int, scale: float = 1.0, dtype=torch.flo
         _bad("vocab and d must be below 2^31")
     _same(index, dout, "dout")
     dout, ld = _rows(dout, n, d, "dout")
-    given = _given(out)
+    given = out
     if out is None:
         if accumulate:
             _bad("accumulate needs out")
@@ -279,9 +270,11 @@ def mingru_scan(zh, h0=None, lengths=None, out=None, h_last=None, save_states: b
     Calls of up to 8 positions give the same bits however a sequence is cut
     into them; a longer one agrees with them to rounding only.  An encoder and
     a decoder that must agree both step in calls of at most 8."""
-    _no_graph("zh h0 out h_last", zh, h0, out, h_last)
+    if (zh.requires_grad or (h0 is not None and h0.requires_grad) or (out is not None and out.requires_grad) or
+            (h_last is not None and h_last.requires_grad) or forward_ad._current_level >= 0):
+        _no_graph("zh h0 out h_last", zh, h0, out, h_last)
     zh, B, T, d, zr, zc, index = _gates(zh)
-    given = _given(out, h_last)
+    given, state = out, h_last
     out, hr, hc = _result(out, zh, (B, T, d), index, "out")
     h0 = _state(h0, (B, d), index, "h0")
     if h_last is None:
@@ -293,6 +286,8 @@ def mingru_scan(zh, h0=None, lengths=None, out=None, h_last=None, save_states: b
     states = zh.new_empty(L.boa_mingru_states_floats(B, T, d), dtype=_FLOAT) if save_states else None
     _call(L.boa_mingru_scan, index, given, zh.data_ptr(), _type(zh, "zh"), zr, zc, B, T, d, _ptr(lengths), _ptr(h0),
           out.data_ptr(), hr, hc, h_last.data_ptr(), _ptr(states))
+    if state is not None:
+        increment_version(state)
     return (out, h_last, states) if save_states else (out, h_last)
 
 
@@ -300,7 +295,10 @@ def mingru_scan_backward(zh, states, dh, dh_last=None, lengths=None, out=None):
     """Gradient of ``mingru_scan`` from dh [chunks, positions, d] (zh's dtype)
     and dh_last fp32 [chunks, d] (None = zeros), with the states its forward
     call saved.  -> (dzh like zh, dh0 fp32 [chunks, d])"""
-    _no_graph("zh states dh dh_last out", zh, states, dh, dh_last, out)
+    if (zh.requires_grad or states.requires_grad or dh.requires_grad or
+            (dh_last is not None and dh_last.requires_grad) or (out is not None and out.requires_grad) or
+            forward_ad._current_level >= 0):
+        _no_graph("zh states dh dh_last out", zh, states, dh, dh_last, out)
     zh, B, T, d, zr, zc, index = _gates(zh)
     if dh.shape != (B, T, d) or dh.dtype != zh.dtype:
         _bad(f"dh must be {zh.dtype} of shape ({B}, {T}, {d})")
@@ -310,7 +308,7 @@ def mingru_scan_backward(zh, states, dh, dh_last=None, lengths=None, out=None):
     if states.dtype != _FLOAT or states.numel() != L.boa_mingru_states_floats(B, T, d) or not states.is_contiguous():
         _bad("states must be what mingru_scan(..., save_states=True) returned for these sizes")
     _same(index, states, "states")
-    given = _given(out)
+    given = out
     out, dr, dc = _result(out, zh, (B, T, 2 * d), index, "out")
     dh_last = _state(dh_last, (B, d), index, "dh_last")
     dh0 = zh.new_empty((B, d), dtype=_FLOAT)
@@ -328,7 +326,9 @@ def token_loss(logits, targets, inv_temperature: float = 1.0, grad_scale: float 
     The gradient is formed when grad_scale, dloss or out is given: that of
     sum(grad_scale * dloss * loss), with dloss fp32 [...] (None = ones), in the
     logits' dtype, in `out` when given (which may be `logits`)."""
-    _no_graph("logits dloss out", logits, dloss, out)
+    if (logits.requires_grad or (dloss is not None and dloss.requires_grad) or
+            (out is not None and out.requires_grad) or forward_ad._current_level >= 0):
+        _no_graph("logits dloss out", logits, dloss, out)
     targets, tok, index = _tokens(targets, "targets")
     if logits.dim() < 1 or logits.shape[:-1] != targets.shape:
         _bad(f"logits {tuple(logits.shape)} do not match targets {tuple(targets.shape)}")
@@ -338,7 +338,7 @@ def token_loss(logits, targets, inv_temperature: float = 1.0, grad_scale: float 
     _same(index, logits, "logits")
     rows, ld = _rows(logits, n, vocab, "logits")
     loss = targets.new_empty(targets.shape, dtype=_FLOAT)
-    grad, ld_grad, given = None, 0, _given(out)
+    grad, ld_grad, given = None, 0, out
     if dloss is not None:
         if dloss.get_device() != index or dloss.dtype != _FLOAT or dloss.shape != targets.shape:
             _bad(f"dloss must be float32 of shape {tuple(targets.shape)} on cuda:{index}")
