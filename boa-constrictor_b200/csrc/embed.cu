@@ -16,8 +16,8 @@
 // same bits.
 //
 // Measured on a B200: 1M x 256 fp32 lookup 148 us (7.2 TB/s of stores); its
-// gradient 191 us; profiled one by one, the row sums take 169 us (6.4 TB/s) and
-// the sort's three launches 28 us.
+// gradient 191 us; profiled one by one, the row sums take 167 us (6.4 TB/s) and
+// the sort's three launches 26 us.  bf16: 115 us (floor 82).
 #include "pieces.h"
 #include "ptx.cuh"
 #include "train_ops.cuh"
@@ -531,8 +531,12 @@ embed_sum_kernel(const TG* __restrict__ dout, long long ld, int d, int per_row, 
   }
 }
 
-// Few rows: one kernel instead of four (4096 x 256: 11 us against 41 us; when
-// all are the same token 40 us against 44 us).  A block takes `per` tokens and up to kSmallPacks packs
+// Few rows: one kernel instead of the cluster's sort and the sums.  On the GPU,
+// fp32 rows spread over 256 tokens: 1024 x 64 4.8 us against 10.3, 4096 x 256 8.2
+// against 11.3, 8192 x 256 11.5 against 11.6.  It is the slower one where few blocks
+// have the work (4096 rows of one token 37 against 14) and for large alphabets
+// (4096 x 160 bf16 over 1000 tokens 23 against 15); the rule sees the number of
+// rows alone.  A block takes `per` tokens and up to kSmallPacks packs
 // of columns; it reads all tokens into shared memory, and for each of its own
 // tokens lists the positions in order (a lane keeps the match mask of every
 // 32 positions of its warp's part) and sums their rows.

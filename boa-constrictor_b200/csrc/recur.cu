@@ -29,12 +29,14 @@
 // cluster, and the result does not depend on timing.
 //
 // Measured on a B200 (floor: the bytes at the 6561 GB/s of a copy).  Many 32-bit
-// chains run at the memory's rate: 256 x 1024 x 256 forward 146 us (0.84),
-// backward 247 us (0.83).  16-bit rows are paced by instruction issue, 35 a value
-// forward and 62 backward: 64 x 4096 x 256 bf16 102 us (0.60) and 166 us (0.61).
+// chains run at the memory's rate: 256 x 1024 x 256 forward 142 us (0.87),
+// backward 245 us (0.84).  16-bit rows are paced by instruction issue, 30 a value
+// forward and 56 backward: 64 x 4096 x 256 bf16 105 us (0.58) and 171 us (0.60);
+// their 256 blocks also leave 40 of the SMs with one instead of two.
 // Few chains are paced by the SMs that clusters reach: 1 x 262144 x 512 fp32
-// 392 us (0.63) and 673 us (0.61).  One position, 16384 x 256: 13.8 and 14.4 us
-// in two captures (0.93, 0.89).
+// 383 us (0.64) and 680 us (0.60).  One position, 16384 x 256: 13.5 to 14.4 us
+// in four captures (0.95 to 0.89); 8 positions 68 us (0.98).  Backward one to
+// eight positions take the walk too: 162 and 178 us (0.11, 0.60).
 #include "ptx.cuh"
 #include "train_ops.cuh"
 
@@ -853,8 +855,8 @@ static size_t grad_smem(int threads, int ranks) {
          (size_t)packs_of_team<G>(kStages, 3, kGradSteps) * (threads / G) * sizeof(Pack<E, V>);
 }
 // Half-warp teams make twice the groups.  They are taken where more SMs then
-// have work (1 x 262144 x 512 fp32 forward: 16 clusters of 6, 473 us, against
-// 32 of 4, 392 us; 1 x 65536 x 64: 95 us and 56 us), not where as many have
+// have work (as first measured, 1 x 262144 x 512 fp32 forward: 16 clusters of 6,
+// 473 us, against 32 of 4, 392 us; 1 x 65536 x 64: 95 us and 56 us), not where as many have
 // (4 x 16384 x 256: 53 us and 58 us).
 static bool half_reaches_further(const Shape& half, const Shape& warp) {
   return half.reach <= 148 && half.reach > warp.reach;

@@ -3,9 +3,12 @@ fp32 arithmetic may be off by, used by the tests of boa_b200.training.
 
 The bounds are running error bounds: each is evaluated next to the value, from
 the documented errors of what the kernels call (u = 2^-24, half a step of
-fp32): __expf(x) 2 + 1.173 |x| steps of 2^-23, __fdividef 2 steps, logf 1
-step, one u for each product and sum.  They hold for any order of the sums
-and any grouping of the recurrence."""
+fp32): ex2.approx 2 steps of 2^-23 and rcp.approx 1, logf 1 step, one u for
+each product and sum.  exp(x) is ex2 of x times log2 e, whose constant and
+product are off by one u each: |x| (2 u) more, below the 1.173 |x| steps of
+2^-23 that are allowed for.  They hold for any order of the sums and any grouping of the
+recurrence.  What an open gate leaves of the state is bounded more closely in
+test_gpu_training_gates.py."""
 import numpy as np
 
 U = 2.0 ** -24
@@ -40,7 +43,8 @@ def embed_grad(tok, dout, vocab, scale):
     out, size = np.zeros((vocab, dout.shape[1])), np.zeros((vocab, dout.shape[1]))
     np.add.at(out, tok[ok], dout[ok])
     np.add.at(size, tok[ok], np.abs(dout[ok]))
-    # at most 512 rows and 256 partial sums are added one after the other in fp32
+    # at most 768 additions one after the other in fp32: the rows of a piece (128 in calls of this size), the
+    # groups of a block and the pieces of a token (at most 256 each)
     return out * scale, (768 * U) * size * abs(scale) + 2 * U * np.abs(out * scale)
 
 
@@ -67,7 +71,7 @@ def mingru(zh, h0, lengths, dh=None, dlast=None):
     for t in range(T):
         h[t + 1] = a[:, t] * h[t] + z[:, t] * c[:, t]
         size[t + 1] = a[:, t] * size[t] + z[:, t] * np.abs(c[:, t])
-        # a is formed as 1 - z: its error is that of z, not relative to a
+        # a's error is taken as that of 1 - z, not relative to a
         err[t + 1] = a[:, t] * err[t] + k[:, t] * (size[t + 1] + z[:, t] * size[t])
     out = np.where(live, h[1:].transpose(1, 0, 2), 0.0)
     got = {"h": (out, np.where(live, err[1:].transpose(1, 0, 2), 0.0)), "last": (h[T], err[T])}
