@@ -1,7 +1,7 @@
 // ptx.cuh -- thin inline-PTX wrappers for sm_100a: mbarriers, TMA bulk-tensor
-// loads, tcgen05 (TMEM alloc, UMMA issue/commit, TMEM loads) and bounded waits.
+// loads, tcgen05 (TMEM alloc, UMMA issue/commit, TMEM loads).
 //
-// Every wait of this library is bounded by the global nanosecond timer.  The
+// Every wait of this library is bounded by the global nanosecond timer; the
 // waits that record a timeout in the device error word are in devword.cuh.
 #pragma once
 #include <cstdint>
